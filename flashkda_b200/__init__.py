@@ -11,8 +11,12 @@ import os
 import torch
 
 from . import _lib
+from .attention import (latent_attention_decode, latent_attention_fwd, latent_decode_workspace_size, linear_attention_fwd,
+                        linear_attention_workspace_size, operator_status)
 
-__all__ = ["fwd", "get_workspace_size", "last_launch_count", "default_algo", "device_status", "chunk_states_slots"]
+__all__ = ["fwd", "get_workspace_size", "last_launch_count", "default_algo", "device_status", "chunk_states_slots",
+           "linear_attention_fwd", "linear_attention_workspace_size", "latent_attention_fwd", "latent_attention_decode",
+           "latent_decode_workspace_size", "operator_status"]
 
 D = 128
 _ENV_ALGO = "FLASHKDA_B200_ALGO"
@@ -91,5 +95,5 @@ def device_status(workspace: torch.Tensor) -> int:
 
 
 def last_launch_count() -> int:
-    """Kernels launched by the last successful ``fwd`` on this thread."""
+    """Kernels launched by the last successful call of an operator on this thread."""
     return int(_lib.lib().fkda_last_launch_count())

@@ -32,6 +32,29 @@ class FwdParams(ctypes.Structure):
     ]
 
 
+class LinearParams(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "g", "out", "initial_state", "final_state", "cu_seqlens")] + \
+               [(n, ctypes.c_int64) for n in ("B", "T", "H", "Hk", "N")] + \
+               [(n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "out_stride", "g_stride")] + \
+               [("scale", ctypes.c_float), ("state_dtype", ctypes.c_int32), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_size_t)]
+
+
+class LatentParams(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "k_rope", "v", "out", "lse", "cu_seqlens", "cu_seqlens_k")] + \
+               [(n, ctypes.c_int64) for n in ("B", "T", "Tk", "H", "N")] + \
+               [(n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] + \
+               [("k_rope_stride", ctypes.c_int64 * 2), ("scale", ctypes.c_float), ("causal", ctypes.c_int32)]
+
+
+class LatentDecodeParams(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "cache", "block_table", "cache_lens", "out", "lse")] + \
+               [(n, ctypes.c_int64) for n in ("B", "Tq", "H", "pages", "page_size", "max_pages")] + \
+               [(n, ctypes.c_int64 * 2) for n in ("q_stride", "out_stride", "cache_stride")] + \
+               [("block_table_stride", ctypes.c_int64), ("scale", ctypes.c_float), ("reserved", ctypes.c_int32),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
 _lib = None
 
 
@@ -65,6 +88,15 @@ def lib():
         L.fkda_device_status.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
         L.fkda_cp_fold.restype = ctypes.c_int
         L.fkda_cp_fold.argtypes = [ctypes.c_void_p] * 4 + [ctypes.c_int64, ctypes.c_void_p]
+        for name, params in (("linear_attention_fwd", LinearParams), ("latent_attention_fwd", LatentParams),
+                             ("latent_attention_decode", LatentDecodeParams)):
+            getattr(L, "fkda_" + name).restype = ctypes.c_int
+            getattr(L, "fkda_" + name).argtypes = [ctypes.POINTER(params), ctypes.c_void_p]
+        for name, params in (("linear", LinearParams), ("latent_decode", LatentDecodeParams)):
+            getattr(L, f"fkda_{name}_workspace_bytes").restype = ctypes.c_size_t
+            getattr(L, f"fkda_{name}_workspace_bytes").argtypes = [ctypes.POINTER(params)]
+        L.fkda_operator_status.restype = ctypes.c_int
+        L.fkda_operator_status.argtypes = [ctypes.c_void_p]
         _lib = L
     return _lib
 

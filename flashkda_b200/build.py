@@ -1,7 +1,7 @@
 """In-tree build of the native parts: ``python -m flashkda_b200.build``.
 
 ``libflashkda_b200.so``: the CUDA library behind the C ABI, plain ``nvcc`` for sm_100a only, no third-party headers.
-``_host.so``: the host side of ``fwd`` (argument checks, scratch, the call of the C ABI), a CPython extension against the
+``_host.so``: the host side of the operators (argument checks, scratch, the calls of the C ABI), a CPython extension against the
 installed PyTorch's headers, plain ``g++``.  Both sit next to this file (git-ignored).
 """
 import glob
@@ -13,7 +13,8 @@ import sysconfig
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libflashkda_b200.so")
-HOST_SRC = os.path.join(CSRC, "fkda_host.cpp")
+HOST_SRC = [os.path.join(CSRC, "fkda_host.cpp"), os.path.join(CSRC, "fkda_host_ops.cpp")]
+HOST_HEADER = os.path.join(CSRC, "fkda_host_args.h")
 HOST = os.path.join(HERE, "_host.so")
 
 NVCC_FLAGS = [
@@ -21,6 +22,7 @@ NVCC_FLAGS = [
     "-ftz=true",  # the reference is built with --use_fast_math; only its flush-to-zero part is numerically
                   # visible in the instruction sequences used here
     "-Xcompiler", "-fPIC", "-shared", "-Xlinker", "-soname=libflashkda_b200.so",
+    "--threads", "0",   # the files beside one another
 ]
 
 
@@ -62,7 +64,7 @@ def _host_command():
            os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}"] +
-            [x for d in inc for x in ("-isystem", d)] + ["-o", HOST, HOST_SRC, LIB, "-L" + os.path.join(root, "lib"),
+            [x for d in inc for x in ("-isystem", d)] + ["-o", HOST] + HOST_SRC + [LIB, "-L" + os.path.join(root, "lib"),
              "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"])
 
 
@@ -71,7 +73,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         nvcc = os.environ.get("NVCC", "nvcc")
         _run([nvcc] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-o", LIB] + sources(),
              "libflashkda_b200.so", verbose)
-    if force or _stale(HOST, [HOST_SRC, LIB] + _headers()):
+    if force or _stale(HOST, HOST_SRC + [HOST_HEADER, LIB] + _headers()):
         _run(_host_command(), "_host.so", verbose)
     return LIB
 

@@ -8,9 +8,11 @@ thread_local int g_last_launches = 0;
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 }  // namespace
 
+void fkda::set_last_launch_count(int n) { g_last_launches = n; }
+
 extern "C" {
 
-int fkda_version(void) { return 1001; }
+int fkda_version(void) { return 1002; }
 
 size_t fkda_params_size(void) { return sizeof(fkda_fwd_params); }
 
@@ -28,6 +30,7 @@ const char* fkda_status_string(int status) {
         case FKDA_ERR_DEVICE_STATUS: return "a kernel reported an internal time-out";
         case FKDA_ERR_NOALLOC_TOO_LARGE:
             return "problem too large for the built-in scratch of fkda_fwd_noalloc (use fkda_fwd with a workspace)";
+        case FKDA_ERR_BAD_SCALE: return "scale must be positive and finite";
         default: return "unknown status";
     }
 }

@@ -24,49 +24,11 @@
 #include <optional>
 #include <string>
 
-#include "../../include/flashkda_b200.h"
+#include "fkda_host_args.h"
+
+using namespace fkda_host;
 
 namespace {
-
-struct Refused : std::runtime_error {
-    using std::runtime_error::runtime_error;
-};
-inline void check(bool ok, const char* msg) {
-    if (!ok) throw Refused(msg);
-}
-inline void check_named(bool ok, const char* name, const char* msg) {
-    if (!ok) throw Refused(std::string(name) + msg);
-}
-
-const at::Tensor& tensor_arg(PyObject* o, const char* name) {
-    if (!THPVariable_Check(o)) throw Refused(std::string(name) + " must be a torch.Tensor");
-    return THPVariable_Unpack(o);
-}
-const at::Tensor* optional_tensor_arg(PyObject* o, const char* name) { return o == Py_None ? nullptr : &tensor_arg(o, name); }
-
-// Whatever float() takes: numpy scalars, one-element tensors, strings.
-double number_arg(PyObject* o) {
-    if (PyFloat_Check(o)) return PyFloat_AS_DOUBLE(o);
-    PyObject* f = PyNumber_Float(o);
-    if (f == nullptr) throw std::bad_cast();
-    const double x = PyFloat_AS_DOUBLE(f);
-    Py_DECREF(f);
-    return x;
-}
-// Whatever int() takes.
-long integer_arg(PyObject* o) {
-    if (PyLong_Check(o)) {
-        const long x = PyLong_AsLong(o);
-        if (x == -1 && PyErr_Occurred()) throw std::bad_cast();
-        return x;
-    }
-    PyObject* i = PyNumber_Long(o);
-    if (i == nullptr) throw std::bad_cast();
-    const long x = PyLong_AsLong(i);
-    Py_DECREF(i);
-    if (x == -1 && PyErr_Occurred()) throw std::bad_cast();
-    return x;
-}
 
 int algo_arg(PyObject* o) {
     const int given = PyObject_IsTrue(o);
@@ -83,11 +45,6 @@ int algo_arg(PyObject* o) {
     if (std::strcmp(s, "tc") == 0) return FKDA_ALGO_TC;
     PyErr_SetString(PyExc_KeyError, s);
     throw std::bad_cast();
-}
-
-bool shape_is(const at::Tensor& t, std::initializer_list<int64_t> want) {
-    const auto s = t.sizes();
-    return s.size() == want.size() && std::equal(want.begin(), want.end(), s.begin());
 }
 
 // Whether the allocator can hand out a scratch of `bytes`, up to a gigabyte, that a call can do without, and nobody else pays for it.
@@ -254,35 +211,19 @@ void fwd_checked(PyObject* const* a) {
         throw Refused(std::string("fkda_fwd failed: ") + fkda_status_string(rc) + " (status " + std::to_string(rc) + ")");
 }
 
-PyObject* host_fwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
-    if (n != 19) {
-        PyErr_SetString(PyExc_TypeError, "fwd takes 19 arguments");
-        return nullptr;
-    }
-    try {
-        fwd_checked(args);
-    } catch (const std::bad_cast&) {
-        if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "fwd: an argument has the wrong type");
-        return nullptr;
-    } catch (const c10::OutOfMemoryError& e) {
-        PyObject* torch = PyImport_ImportModule("torch");
-        PyObject* cls = torch != nullptr ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
-        PyErr_SetString(cls != nullptr ? cls : PyExc_RuntimeError, e.what_without_backtrace());
-        Py_XDECREF(cls);
-        Py_XDECREF(torch);
-        return nullptr;
-    } catch (const std::exception& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
-        return nullptr;
-    }
-    Py_RETURN_NONE;
-}
+PyObject* host_fwd(PyObject*, PyObject* const* args, Py_ssize_t n) { return refusing("fwd", 19, n, [&] { fwd_checked(args); }); }
 
 PyMethodDef methods[] = {
     {"fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(host_fwd)), METH_FASTCALL,
      "Checks the arguments of one forward call and enqueues it (see flashkda_b200.fwd)."},
+    {"linear_attention_fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(host_linear_attention_fwd)), METH_FASTCALL,
+     "Checks the arguments of one call and enqueues it (see flashkda_b200.linear_attention_fwd)."},
+    {"latent_attention_fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(host_latent_attention_fwd)), METH_FASTCALL,
+     "Checks the arguments of one call and enqueues it (see flashkda_b200.latent_attention_fwd)."},
+    {"latent_attention_decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(host_latent_attention_decode)), METH_FASTCALL,
+     "Checks the arguments of one call and enqueues it (see flashkda_b200.latent_attention_decode)."},
     {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "Native host side of flashkda_b200.fwd.", -1, methods,
+PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "Native host side of flashkda_b200.fwd and of the operators beside it.", -1, methods,
                           nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

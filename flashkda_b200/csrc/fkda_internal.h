@@ -90,6 +90,19 @@ int launch_short(const fkda_fwd_params& p, cudaStream_t stream, int* n_launches)
 // the prefix kernel decides on the device), and the launch of the fused kernel behind that decision.
 bool short_ragged_candidate(const fkda_fwd_params& p);
 int launch_short_ragged(const fkda_fwd_params& p, const TwoPassArgs& a, cudaStream_t stream);
+// A tensor map over bf16 data, innermost dimension first (strides in bytes, of the dimensions from the second on), 128-byte
+// swizzle (fkda_tc.cu).
+bool encode_bf16_map(CUtensorMap* m, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box);
+// Linear and latent attention.
+size_t linear_workspace(const fkda_linear_params& p);
+int launch_linear(const fkda_linear_params& p, cudaStream_t stream, int* n_launches);
+int launch_latent_prompt(const fkda_latent_params& p, cudaStream_t stream, int* n_launches);
+size_t latent_decode_workspace(const fkda_latent_decode_params& p);
+int launch_latent_decode(const fkda_latent_decode_params& p, cudaStream_t stream, int* n_launches);
+int linear_gave_up(cudaStream_t stream, int32_t* word);   // of the waits in each file's kernels
+int prompt_gave_up(cudaStream_t stream, int32_t* word);
+int decode_gave_up(cudaStream_t stream, int32_t* word);
+void set_last_launch_count(int n);
 // Tensor maps over v and over the states (fkda_tc.cu).
 bool encode_v_map(CUtensorMap* m, const fkda_fwd_params& p);
 bool encode_state_map(CUtensorMap* m, const void* base, int64_t chains, bool fp32);

@@ -1,0 +1,374 @@
+// Latent attention, expanded form: every head has keys of its own for the 128 unrotated dimensions and values of its own, and
+// shares the 64 rotated ones of the token.  For a prompt:
+//     o_i = sum_j softmax_j(scale (q_i[0:128] . k_j + q_i[128:192] . r_j)) v_j
+//
+// One pass over the keys with the running maximum and sum of the softmax.  A CTA serves 256 rows of one head as two tiles of
+// 128, each with a warpgroup of its own that turns scores into weights, one row per thread; while one tile's weights are being made
+// the tensor cores work for the other.  Scores and outputs live in tensor memory (2 x 128 + 2 x 128 columns), the weights
+// overwrite the scores as the A operand of the product with v.  Keys and values come through a ring of eight 16 KB tiles
+// (128 tokens x 64 dimensions); the rotated part needs no copy beside the others: it is the third tile of a key block, read
+// through a map of its own.
+//
+// Numerics: products of bf16 with fp32 sums, weights relative to a reference that follows the running maximum once that is
+// 2^8 above it (so weights stay below 2^8 and the sums are exact to 32 bits either way), weights rounded to bf16 for the product
+// with v (their relative error, 2^-9 at most, averages out over the keys; the sum and lse use the unrounded weights).
+#include "fkda_tc5.cuh"
+
+namespace fkda {
+namespace {
+
+using namespace tc5;
+
+constexpr int kTile = 128;                   // query rows of a warpgroup, and keys of a block
+constexpr int kRows = 2 * kTile;             // query rows of a CTA
+constexpr int kSlotBytes = kTile * 128;      // 128 tokens x 64 dimensions
+constexpr int kSlots = 8;
+constexpr int kKeyTiles = 3, kValueTiles = 2;
+constexpr int kThreads = 320;                // two softmax warpgroups, a loading and a multiplying warp
+constexpr int kSmem = 1024 + (2 * kKeyTiles + kSlots) * kSlotBytes + 256;
+constexpr uint32_t kS = 0, kO = 256;         // tensor-memory columns: scores (and weights) of the two tiles, outputs
+
+struct PromptMaps {
+    CUtensorMap q, k, r, v;
+};
+struct PromptArgs {
+    __nv_bfloat16* out;
+    float* lse;
+    const int64_t *cu_q, *cu_k;
+    int64_t B, T, Tk, N, out_batch, out_token, out_head;
+    int H;
+    float scale;
+    int causal;
+};
+
+struct Bars {
+    uint64_t q_full, full[kSlots], empty[kSlots], s_full[2], p_full[2], o_done[2], drained;
+    uint32_t tmem;
+    int abort;
+};
+
+// Where a CTA's rows are: sequence, first row, and the extents of queries and keys.
+struct Place {
+    int64_t q0, k0, b;     // first token of the sequence's queries and keys, batch row
+    int len_q, len_k, row0;
+    bool any;
+};
+__device__ __forceinline__ Place locate(const PromptArgs& a, int64_t slot, int lane) {
+    Place p;
+    if (a.cu_q == nullptr) {
+        // long rows first: the last block of every sequence, then the one in front of it, ...
+        const int64_t tiles = (a.T + kRows - 1) / kRows, t = slot / a.N;
+        p.b = slot - t * a.N;
+        p.q0 = p.k0 = 0;
+        p.len_q = (int)a.T;
+        p.len_k = (int)a.Tk;
+        p.row0 = (int)(tiles - 1 - t) * kRows;
+        p.any = true;
+        return p;
+    }
+    int64_t seen = 0;
+    p.any = false;
+    p.b = 0;
+    for (int64_t base = 0; base < a.N; base += 32) {
+        const int64_t n = base + lane;
+        int64_t lo = 0, len = 0;
+        if (n < a.N) {
+            lo = a.cu_q[n] < 0 ? 0 : a.cu_q[n];
+            const int64_t hi = a.cu_q[n + 1] > a.T ? a.T : a.cu_q[n + 1];
+            len = hi > lo ? hi - lo : 0;
+        }
+        const int tiles = (int)((len + kRows - 1) / kRows);
+        int upto = tiles;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, off);
+            if (lane >= off) upto += x;
+        }
+        const uint32_t behind = __ballot_sync(0xffffffffu, seen + upto > slot);
+        if (behind != 0) {
+            const int src = __ffs(behind) - 1;
+            const int64_t first = seen + __shfl_sync(0xffffffffu, upto - tiles, src);
+            const int64_t seq = base + src;
+            p.q0 = __shfl_sync(0xffffffffu, lo, src);
+            p.len_q = (int)__shfl_sync(0xffffffffu, len, src);
+            p.row0 = (int)((p.len_q + kRows - 1) / kRows - 1 - (slot - first)) * kRows;
+            const int64_t klo = a.cu_k[seq] < 0 ? 0 : a.cu_k[seq], khi = a.cu_k[seq + 1] > a.Tk ? a.Tk : a.cu_k[seq + 1];
+            p.k0 = klo;
+            p.len_k = khi > klo ? (int)(khi - klo) : 0;
+            p.any = true;
+            return p;
+        }
+        seen += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return p;
+}
+
+__global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ PromptMaps maps) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* q_smem = smem;                                        // [2 tiles][3][128 rows][128 bytes]
+    uint8_t* ring = smem + 2 * kKeyTiles * kSlotBytes;
+    Bars& bar = *reinterpret_cast<Bars*>(ring + kSlots * kSlotBytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(&bar.q_full, 1);
+        for (int i = 0; i < kSlots; ++i) mbar_init(&bar.full[i], 1), mbar_init(&bar.empty[i], 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&bar.s_full[i], 1), mbar_init(&bar.p_full[i], kTile), mbar_init(&bar.o_done[i], 1);
+        mbar_init(&bar.drained, 1);
+        bar.abort = 0;
+        mbar_fence_init();
+    }
+    if (warp == 9) tmem_alloc(&bar.tmem, 512);
+    fence_before();
+    grid_dep_launch();
+    grid_dep_wait();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = bar.tmem;
+    const Place p = locate(a, blockIdx.x / a.H, lane);
+    const int h = (int)(blockIdx.x % a.H);
+    // key blocks of the two tiles: a row sees the keys up to its own place counted from the ends
+    int n[2] = {0, 0};
+    if (p.any) {
+        for (int w = 0; w < 2; ++w) {
+            const int last = min(p.row0 + (w + 1) * kTile, p.len_q);   // one past the tile's last row
+            if (p.row0 + w * kTile >= p.len_q) continue;
+            const int seen = a.causal ? min(p.len_k, max(0, p.len_k - p.len_q + last)) : p.len_k;
+            n[w] = (seen + kTile - 1) / kTile;
+        }
+    }
+    const int blocks = max(n[0], n[1]);
+
+    if (warp == 8) {
+        // ---- loads: the queries, then for every block its keys (two tiles of the head's, one of the token's) and values ----
+        if (blocks > 0 && elect_one()) {
+            mbar_arrive_expect_tx(&bar.q_full, 2 * kKeyTiles * kSlotBytes);
+            for (int w = 0; w < 2; ++w)
+                for (int c = 0; c < kKeyTiles; ++c)
+                    tma_load_4d(q_smem + (w * kKeyTiles + c) * kSlotBytes, &maps.q, c * 64, h, (int)(p.q0 + p.row0 + w * kTile), (int)p.b, &bar.q_full);
+            int s = 0;
+            bool ok = true;
+            for (int i = 0; i < blocks && ok; ++i) {
+                const int t = (int)p.k0 + i * kTile;
+                for (int c = 0; c < kKeyTiles + kValueTiles && ok; ++c, ++s) {
+                    const int slot = s % kSlots;
+                    if (s >= kSlots) ok = wait(&bar.empty[slot], (s / kSlots - 1) & 1, &bar.abort);
+                    if (!ok) break;
+                    uint8_t* dst = ring + slot * kSlotBytes;
+                    mbar_arrive_expect_tx(&bar.full[slot], kSlotBytes);
+                    if (c < 2) tma_load_4d(dst, &maps.k, c * 64, h, t, (int)p.b, &bar.full[slot]);
+                    else if (c == 2) tma_load_3d(dst, &maps.r, 0, t, (int)p.b, &bar.full[slot]);
+                    else tma_load_4d(dst, &maps.v, (c - 3) * 64, h, t, (int)p.b, &bar.full[slot]);
+                }
+            }
+            drain(&bar.q_full, 0);
+            for (int k = max(0, s - kSlots); k < s; ++k) drain(&bar.full[k % kSlots], (k / kSlots) & 1);
+        }
+    } else if (warp == 9) {
+        // ---- products ----
+        if (blocks > 0 && elect_one()) {
+            constexpr uint32_t kIdS = idesc(kTile, kTile, false, false), kIdO = idesc(kTile, kTile, false, true);
+            const uint32_t q_addr = smem_u32(q_smem), ring_addr = smem_u32(ring);
+            constexpr int kEach = kKeyTiles + kValueTiles;
+            bool ok = wait(&bar.q_full, 0, &bar.abort);
+            auto scores = [&](int w, int i, bool first) {   // tile w against key block i
+                for (int c = 0; c < kKeyTiles; ++c) {
+                    const int s = i * kEach + c;
+                    if (first && ok) ok = wait(&bar.full[s % kSlots], (s / kSlots) & 1, &bar.abort);
+                    fence_after();
+                    for (int k = 0; k < 4; ++k)
+                        mma_ss(tmem + kS + w * kTile, desc(q_addr + (w * kKeyTiles + c) * kSlotBytes + k * 32),
+                               desc(ring_addr + (s % kSlots) * kSlotBytes + k * 32), kIdS, (c | k) != 0);
+                }
+                commit(&bar.s_full[w]);
+            };
+            auto free_slots = [&](int first, int count) {
+                for (int s = first; s < first + count; ++s) commit(&bar.empty[s % kSlots]);
+            };
+            for (int w = 0; w < 2; ++w)
+                if (n[w] > 0 && ok) scores(w, 0, w == 0 || n[0] == 0);
+            free_slots(0, kKeyTiles);
+            for (int i = 0; i < blocks && ok; ++i) {
+                const int first_v = i < n[0] ? 0 : 1, last_v = i < n[1] ? 1 : 0;
+                const int first_k = i + 1 < n[0] ? 0 : 1, last_k = i + 1 < n[1] ? 1 : 0;
+                for (int w = 0; w < 2 && ok; ++w) {
+                    if (i >= n[w]) continue;
+                    ok = wait(&bar.p_full[w], i & 1, &bar.abort);
+                    if (!ok) break;
+                    for (int c = 0; c < kValueTiles && w == first_v && ok; ++c) {
+                        const int s = i * kEach + kKeyTiles + c;
+                        ok = wait(&bar.full[s % kSlots], (s / kSlots) & 1, &bar.abort);
+                    }
+                    if (!ok) break;
+                    fence_after();
+                    for (int c = 0; c < kValueTiles; ++c) {   // N = 64 dimensions at a time: the two tiles need not be neighbours in the ring
+                        const uint32_t v_addr = ring_addr + ((i * kEach + kKeyTiles + c) % kSlots) * kSlotBytes;
+                        for (int k = 0; k < 8; ++k)
+                            mma_ts(tmem + kO + w * kTile + c * 64, tmem + kS + w * kTile + k * 8, desc(v_addr + k * 2048),
+                                   idesc(kTile, 64, false, true), i > 0 || k > 0);
+                    }
+                    commit(&bar.o_done[w]);
+                    if (w == last_v) free_slots(i * kEach + kKeyTiles, kValueTiles);
+                    if (i + 1 < n[w]) {
+                        scores(w, i + 1, w == first_k);
+                        if (w == last_k) free_slots((i + 1) * kEach, kKeyTiles);
+                    }
+                }
+            }
+            (void)kIdO;
+            commit(&bar.drained);
+            drain(&bar.drained, 0);
+        }
+    } else {
+        // ---- weights: thread = row ----
+        const int w = warp >> 2;
+        const int row = p.row0 + w * kTile + (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + kS + w * kTile + lanes, to = tmem + kO + w * kTile + lanes;
+        const float c = a.scale * 1.4426950408889634f;
+        int seen = p.any ? (a.causal ? p.len_k - p.len_q + row + 1 : p.len_k) : 0;
+        seen = min(max(seen, 0), p.any ? p.len_k : 0);
+        const int least = p.any ? (a.causal ? p.len_k - p.len_q + p.row0 + w * kTile + 1 : p.len_k) : 0;   // what the tile's first row sees
+        const float step = 8.0f / c;
+        float top = -INFINITY, sum = 0.0f;
+        uint32_t s[128];
+        for (int i = 0; i < n[w]; ++i) {
+            wait(&bar.s_full[w], i & 1, &bar.abort);
+            fence_after();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) ld32(ts + k * 32, s + k * 32);
+            wait_ld();
+            if ((i + 1) * kTile > least || (i + 1) * kTile > p.len_k) {
+#pragma unroll
+                for (int k = 0; k < 128; ++k) s[k] = i * kTile + k < seen ? s[k] : 0xff800000u;
+            }
+            float m = f(s[0]);
+#pragma unroll
+            for (int k = 1; k < 128; ++k) m = fmaxf(m, f(s[k]));
+            // the reference moves where the maximum is 2^8 above it; then what was summed so far is scaled down
+            const bool move = m > top + step || (top == -INFINITY && m > -INFINITY);
+            if (__any_sync(0xffffffffu, move)) {
+                const float factor = move ? (top == -INFINITY ? 0.0f : ex2_approx((top - m) * c)) : 1.0f;
+                if (move) top = m;
+                sum *= factor;
+                if (i > 0) {   // (the product with the last block's values is complete: the scores were issued behind it)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t o[32];
+                        ld32(to + k * 32, o);
+                        wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = u(f(o[j]) * factor);
+                        st32(to + k * 32, o);
+                    }
+                }
+            }
+            const float ref = top == -INFINITY ? 0.0f : -top * c;
+            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < 128; ++k) {
+                const float e = ex2_approx(__fmaf_rn(f(s[k]), c, ref));
+                part[k & 3] += e;
+                s[k] = u(e);
+            }
+            sum += (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+            for (int k = 0; k < 64; ++k) s[k] = pack_bf2(f(s[2 * k]), f(s[2 * k + 1]));
+            st32(ts, s);
+            st32(ts + 32, s + 32);
+            // values behind the sequence's last key are another sequence's, or nobody's: nothing times them must be nothing
+            if ((i + 1) * kTile > p.len_k && w == (i < n[0] ? 0 : 1)) {
+                const int from = p.len_k - i * kTile;
+                for (int v = 0; v < kValueTiles; ++v) {
+                    const int sl = i * (kKeyTiles + kValueTiles) + kKeyTiles + v;
+                    wait(&bar.full[sl % kSlots], (sl / kSlots) & 1, &bar.abort);
+                    uint4* dst = reinterpret_cast<uint4*>(ring + (sl % kSlots) * kSlotBytes);
+                    for (int k = from * 8 + (threadIdx.x & 127); k < kTile * 8; k += 128) dst[k] = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async_smem();
+            }
+            wait_st();
+            fence_before();
+            arrive(&bar.p_full[w]);
+        }
+        if (n[w] > 0) {
+            wait(&bar.o_done[w], (n[w] - 1) & 1, &bar.abort);
+            fence_after();
+        }
+        const bool mine = p.any && row < p.len_q;
+        const int64_t tok = p.q0 + row;
+        const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);   // (a sum that is not a number stays one)
+        __nv_bfloat16* dst = a.out + p.b * a.out_batch + tok * a.out_token + h * a.out_head;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            uint32_t o[32];
+            if (n[w] > 0) {
+                ld32(to + k * 32, o);
+                wait_ld();
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) o[j] = 0u;
+            }
+            if (mine) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint4 x;
+                    x.x = pack_bf2(f(o[8 * j]) * inv, f(o[8 * j + 1]) * inv);
+                    x.y = pack_bf2(f(o[8 * j + 2]) * inv, f(o[8 * j + 3]) * inv);
+                    x.z = pack_bf2(f(o[8 * j + 4]) * inv, f(o[8 * j + 5]) * inv);
+                    x.w = pack_bf2(f(o[8 * j + 6]) * inv, f(o[8 * j + 7]) * inv);
+                    *reinterpret_cast<uint4*>(dst + k * 32 + j * 8) = x;
+                }
+            }
+        }
+        if (mine && a.lse != nullptr)
+            a.lse[(p.b * a.T + tok) * a.H + h] = sum == 0.0f ? -INFINITY : (top == -INFINITY ? 0.0f : top * a.scale) + logf(sum);
+        fence_before();
+    }
+    __syncthreads();
+    fence_after();
+    if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace
+
+int launch_latent_prompt(const fkda_latent_params& p, cudaStream_t stream, int* n_launches) {
+    PromptMaps maps;
+    auto map4 = [](CUtensorMap* m, const void* base, int64_t d, int64_t h, int64_t t, int64_t b, const int64_t* st) {
+        const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)h, (cuuint64_t)t, (cuuint64_t)b};
+        const cuuint64_t strides[3] = {(cuuint64_t)st[2] * 2, (cuuint64_t)st[1] * 2, (cuuint64_t)st[0] * 2};
+        const cuuint32_t box[4] = {64u, 1u, (cuuint32_t)kTile, 1u};
+        return encode_bf16_map(m, 4, base, dims, strides, box);
+    };
+    const cuuint64_t rdims[3] = {64u, (cuuint64_t)p.Tk, (cuuint64_t)p.B};
+    const cuuint64_t rstrides[2] = {(cuuint64_t)p.k_rope_stride[1] * 2, (cuuint64_t)p.k_rope_stride[0] * 2};
+    const cuuint32_t rbox[3] = {64u, (cuuint32_t)kTile, 1u};
+    if (p.Tk > 0) {
+        if (!map4(&maps.k, p.k, 128, p.H, p.Tk, p.B, p.k_stride) || !map4(&maps.v, p.v, 128, p.H, p.Tk, p.B, p.v_stride) ||
+            !encode_bf16_map(&maps.r, 3, p.k_rope, rdims, rstrides, rbox))
+            return FKDA_ERR_LAUNCH;
+    }
+    if (!map4(&maps.q, p.q, 192, p.H, p.T, p.B, p.q_stride)) return FKDA_ERR_LAUNCH;
+    if (p.Tk == 0) maps.k = maps.v = maps.r = maps.q;   // (no key is read)
+    PromptArgs a;
+    a.out = static_cast<__nv_bfloat16*>(p.out);
+    a.lse = p.lse;
+    a.cu_q = p.cu_seqlens;
+    a.cu_k = p.cu_seqlens_k;
+    a.B = p.B; a.T = p.T; a.Tk = p.Tk; a.N = p.N;
+    a.out_batch = p.out_stride[0]; a.out_token = p.out_stride[1]; a.out_head = p.out_stride[2];
+    a.H = (int)p.H;
+    a.scale = p.scale;
+    a.causal = p.causal;
+    const int64_t tiles = (p.T + kRows - 1) / kRows;
+    const int64_t ctas = (p.cu_seqlens != nullptr ? p.T / kRows + p.N : tiles * p.B) * p.H;   // (ragged: never fewer than there are)
+    if (ctas > 0x7fffffff) return FKDA_ERR_BAD_SHAPE;
+    if (!allow_smem<latent_prompt_kernel>(kSmem)) return FKDA_ERR_LAUNCH;
+    if (!launch_dependent(latent_prompt_kernel, ctas, kThreads, kSmem, stream, a, maps)) return FKDA_ERR_LAUNCH;
+    *n_launches = 1;
+    return FKDA_OK;
+}
+
+int prompt_gave_up(cudaStream_t stream, int32_t* word) { return read_gave_up(stream, word); }
+
+}  // namespace fkda

@@ -250,7 +250,7 @@ static bool encode_map(CUtensorMap* m, CUtensorMapDataType type, int rank, const
                        const cuuint64_t* strides, const cuuint32_t* box) {
     EncodeTiledFn encode = encode_tiled_fn();
     if (encode == nullptr) return false;
-    const cuuint32_t estr[3] = {1u, 1u, 1u};
+    const cuuint32_t estr[5] = {1u, 1u, 1u, 1u, 1u};
     auto encoded = [&]() {
         return encode(m, type, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -261,6 +261,9 @@ static bool encode_map(CUtensorMap* m, CUtensorMapDataType type, int rank, const
         if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) rc = encoded();
     }
     return rc == CUDA_SUCCESS;
+}
+bool encode_bf16_map(CUtensorMap* m, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+    return encode_map(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, base, dims, strides, box);
 }
 // Map over v viewed as [token][head][128] bf16 with tiles of 16 tokens x 64 columns of one head; the 16-byte pieces of a tile
 // row are permuted by the row (128-byte swizzle), so that transposing reads of the tile (8 rows of one piece) do not collide.

@@ -1,0 +1,168 @@
+// Inline-PTX wrappers for tensor memory and tcgen05.mma, and the waits of the kernels that use them (linear and latent
+// attention).
+#pragma once
+
+#include "fkda_common.cuh"
+#include "fkda_internal.h"
+#include "fkda_sm100.cuh"
+
+namespace fkda {
+namespace tc5 {
+
+using namespace sm100;
+
+// ------------------------------------------------------------------ waits ----
+// Every wait of these kernels is bounded.  One that gives up raises the CTA's abort flag, at which the other waits of the CTA
+// return at once: the roles run to their ends on whatever is in shared memory (all accesses in bounds), the copies and
+// products in flight are waited for, tensor memory is freed, and the word below tells the host (fkda_operator_status).
+static __device__ int32_t g_gave_up = 0;
+constexpr uint64_t kWaitNs = 2000000000ull;
+
+// The word of this translation unit's kernels, once the stream has come this far; cleared for the next reader.
+static int read_gave_up(cudaStream_t stream, int32_t* word) {
+    const int32_t zero = 0;
+    if (cudaMemcpyFromSymbolAsync(word, g_gave_up, sizeof(*word), 0, cudaMemcpyDeviceToHost, stream) != cudaSuccess ||
+        cudaStreamSynchronize(stream) != cudaSuccess)
+        return FKDA_ERR_LAUNCH;
+    if (*word != 0 && cudaMemcpyToSymbolAsync(g_gave_up, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, stream) != cudaSuccess) return FKDA_ERR_LAUNCH;
+    return FKDA_OK;
+}
+
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* abort_flag) {
+    if (mbar_wait_bounded(bar, parity, abort_flag, kWaitNs)) return true;
+    *reinterpret_cast<volatile int*>(abort_flag) = 1;
+    g_gave_up = 1;
+    return false;
+}
+// For what is in flight when a role ends: not cut short by the abort flag.
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) { mbar_wait_bounded(bar, parity, nullptr, kWaitNs); }
+
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void named_sync(int id, int threads) {
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+// Barrier among `threads` threads that tells all of them whether any had `x` true.
+__device__ __forceinline__ bool named_any(int id, int threads, bool x) {
+    uint32_t any;
+    asm volatile(
+        "{\n.reg .pred p, q;\nsetp.ne.u32 p, %3, 0;\nbarrier.cta.red.or.pred q, %1, %2, p;\nselp.u32 %0, 1, 0, q;\n}\n"
+        : "=r"(any)
+        : "r"(id), "r"(threads), "r"((uint32_t)x)
+        : "memory");
+    return any != 0;
+}
+
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* tmap, int c0, int c1, int c2, int c3, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+        ::"r"(smem_u32(smem_dst)), "l"(tmap), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// ---------------------------------------------------------- tensor memory ----
+// One full warp allocates `n_cols` (power of two, 32..512) columns; the base address is written to shared memory.  The same
+// warp frees them before the CTA exits.
+__device__ __forceinline__ void tmem_alloc(uint32_t* smem_result, uint32_t n_cols) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_result)), "r"(n_cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t n_cols) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(n_cols) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Each thread reads or writes its own lane (lane field of taddr = 32 * (warp % 4)), 32 consecutive 32-bit columns.
+__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+// Fragment-shaped accesses for accumulators of 64 rows, whose rows 16 w .. 16 w + 15 live in lanes 32 w .. 32 w + 15.  Thread
+// 4 g + t of warp w:
+//   load of 64 columns:   r[4 i], r[4 i + 1] = (row g, columns 8 i + 2 t, + 1), r[4 i + 2], r[4 i + 3] = (row g + 8, the same)
+//   store of 32 columns:  r[2 i] -> (row g, column 4 i + t), r[2 i + 1] -> (row g + 8, column 4 i + t)
+// so 64 fp32 columns that were loaded, rounded to bf16 pairs, are stored as an A operand of 64 rows and K = 64.
+__device__ __forceinline__ void ld_frag64(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void st_frag32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+// ------------------------------------------------------------ tcgen05.mma ----
+// Shared-memory operands are tiles of 128-byte rows (64 bf16), written by tiled copies with the 128-byte swizzle (the 16-byte
+// pieces of row r are permuted by r % 8); tiles start at multiples of 1024 bytes.
+//   K-major operand: a tile row is a row of the operand, the tile's columns are 64 steps of K; 16 steps are 32 bytes of the start
+//     address; groups of 8 rows are 1024 bytes apart.
+//   MN-major operand: a tile row is one step of K, the tile's columns are 64 rows (M or N) of the operand; 16 steps are 2048 bytes
+//     of the start address; `block` is the distance to the tile of the next 64 rows.
+// Fields: start address [0,14), leading distance [16,30), stride of 8-row groups [32,46) (all >> 4), version 1 at bit 46,
+// swizzle mode 2 (128 bytes) at [61,64).
+__device__ __forceinline__ uint64_t desc(uint32_t smem_addr, uint32_t block = 16) {
+    return (uint64_t)((smem_addr >> 4) & 0x3fffu) | (uint64_t)((block >> 4) & 0x3fffu) << 16 | (uint64_t)(1024 >> 4) << 32 |
+           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// Instruction descriptor for bf16 operands and fp32 accumulation: D format [4,6) = 1, A and B formats [7,10), [10,13) = 1, MN-major
+// flags of A and B at bits 15 and 16, N >> 3 at [17,23), M >> 4 at [24,29).
+__host__ __device__ constexpr uint32_t idesc(int M, int N, bool a_mn, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
+           ((uint32_t)(M >> 4) << 24);
+}
+// D[tmem] (+)= A[smem] B[smem], K = 16; issued by ONE thread.  accumulate = 0 overwrites D.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+                 "l"(a), "l"(b), "r"(id), "r"(accumulate)
+                 : "memory");
+}
+// D[tmem] (+)= A[tmem] B[smem]: A sits in tensor memory, two bf16 per 32-bit column (8 columns per instruction).
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+                 "r"(a), "l"(b), "r"(id), "r"(accumulate)
+                 : "memory");
+}
+// The mbarrier completes when all tcgen05.mma issued so far by this thread have.
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ float f(uint32_t x) { return __uint_as_float(x); }
+__device__ __forceinline__ uint32_t u(float x) { return __float_as_uint(x); }
+
+}  // namespace tc5
+}  // namespace fkda

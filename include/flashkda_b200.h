@@ -36,7 +36,8 @@ enum {
     FKDA_ERR_LAUNCH = 7,         /* a kernel launch or CUDA runtime call failed */
     FKDA_ERR_ALIGNMENT = 8,      /* a tensor base address or stride is not 16-byte aligned */
     FKDA_ERR_DEVICE_STATUS = 9,  /* a kernel gave up on a bounded internal wait */
-    FKDA_ERR_NOALLOC_TOO_LARGE = 10 /* problem needs more scratch than fkda_fwd_noalloc has built in */
+    FKDA_ERR_NOALLOC_TOO_LARGE = 10, /* problem needs more scratch than fkda_fwd_noalloc has built in */
+    FKDA_ERR_BAD_SCALE = 11      /* scale must be positive and finite */
 };
 
 enum { FKDA_STATE_BF16 = 0, FKDA_STATE_FP32 = 1 };
@@ -184,7 +185,7 @@ int fkda_fwd_noalloc(const fkda_fwd_params* p, void* stream);
 size_t fkda_noalloc_scratch_bytes(void);
 
 /* Library ABI version (major * 1000 + minor). */
-int fkda_version(void);   /* 1001: fkda_fwd_params gained chunk_states, chunk_states_every */
+int fkda_version(void);   /* 1001: fkda_fwd_params gained chunk_states, chunk_states_every; 1002: linear and latent attention */
 
 /* sizeof(fkda_fwd_params) as compiled into the loaded library: a binding checks its own struct against it. */
 size_t fkda_params_size(void);
@@ -192,7 +193,7 @@ size_t fkda_params_size(void);
 /* Static, human-readable name of a status code. */
 const char* fkda_status_string(int status);
 
-/* Number of kernels the last successful fkda_fwd call on this thread launched. */
+/* Number of kernels the last successful call of an operator on this thread launched. */
 int fkda_last_launch_count(void);
 
 /* Context parallelism (no counterpart in the reference, which has no multi-GPU path): a shard of chunks maps the state
@@ -200,6 +201,84 @@ int fkda_last_launch_count(void);
  * independent [128,128] fp32 row-major matrices: out[i] = S[i] . M[i] + N[i] (N == NULL: no offset), plain fp32 FMAs in
  * the order k = 0 .. 127.  `out` must not alias S or M.  Enqueued on `stream`. */
 int fkda_cp_fold(const float* S, const float* M, const float* N, float* out, int64_t count, void* stream);
+
+/* ---- Operators beside the KDA forward (no counterpart in the reference) ----
+ *
+ * Strides are in elements.  Where a tensor is read in tiles (q, k, v, k_rope, cache) its base address and the strides of its
+ * dimensions longer than one are multiples of 16 bytes, and so are those of out; the innermost dimension is contiguous. */
+
+/*
+ * Linear attention with a decay for each head: S_t = exp(g_t) S_{t-1} + v_t k_t^T, o_t = scale S_t q_t.
+ * q, k bf16 [B,T,Hk,128], v, out bf16 [B,T,H,128], Hk divides H (value head h reads key head h / (H / Hk)); g fp32 [B,T,H], natural
+ * logarithms of the decays (below -100 counts as -100; all strides 0 where one value serves a dimension); states [N,H,128,128]
+ * ([V,K]) contiguous, 16-byte aligned, NULL for none, initial and final may be the same buffer; cu_seqlens int64 [N + 1] (then
+ * B == 1) or NULL (N == B).  Rows that no sequence has are not written.
+ */
+typedef struct fkda_linear_params {
+    const void *q, *k, *v;
+    const float* g;
+    void* out;
+    const void* initial_state;
+    void* final_state;
+    const int64_t* cu_seqlens;
+    int64_t B, T, H, Hk, N;
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3]; /* batch, token, head */
+    int64_t g_stride[3];
+    float scale;
+    int32_t state_dtype; /* FKDA_STATE_BF16 or FKDA_STATE_FP32, of both states */
+    void* workspace;     /* 256-byte aligned; fkda_linear_workspace_bytes() of them */
+    size_t workspace_bytes;
+} fkda_linear_params;
+size_t fkda_linear_workspace_bytes(const fkda_linear_params* p);
+int fkda_linear_attention_fwd(const fkda_linear_params* p, void* stream);
+
+/*
+ * Latent attention, expanded form (prompts): o_i = sum_j softmax_j(scale (q_i[0:128] . k_j + q_i[128:192] . k_rope_j)) v_j.
+ * q bf16 [B,T,H,192], k, v bf16 [B,Tk,H,128], k_rope bf16 [B,Tk,64], out bf16 [B,T,H,128], lse fp32 [B,T,H] contiguous or NULL
+ * (logarithm of the sum, -inf for a row that sees nothing, whose out is 0).  causal: row i of T_n sees the keys j of Tk_n with
+ * j <= i + Tk_n - T_n.  cu_seqlens, cu_seqlens_k int64 [N + 1], both (then B == 1) or neither.
+ */
+typedef struct fkda_latent_params {
+    const void *q, *k, *k_rope, *v;
+    void* out;
+    float* lse;
+    const int64_t *cu_seqlens, *cu_seqlens_k;
+    int64_t B, T, Tk, H, N;
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3]; /* batch, token, head */
+    int64_t k_rope_stride[2];                                     /* batch, token */
+    float scale;
+    int32_t causal;
+} fkda_latent_params;
+int fkda_latent_attention_fwd(const fkda_latent_params* p, void* stream);
+
+/*
+ * Latent attention, absorbed form, over a paged cache: for the Tq newest tokens of every sequence
+ * o_r = sum_j softmax_j(scale q_r . c_j) c_j[0:512], where new token i of Tq sees the cached tokens j < len - Tq + 1 + i.
+ * q bf16 [B,Tq,H,576], out bf16 [B,Tq,H,512] (rows = new token x head, one stride), cache bf16 [pages,page_size,576], page_size a
+ * multiple of 16; block_table int32 [B][max_pages]: page of the tokens page_size i .. page_size (i + 1) - 1; cache_lens int32 [B],
+ * the new tokens among them (a length beyond the table counts as the table's end); lse fp32 [B,Tq,H] contiguous or NULL.
+ * What lies behind a sequence's last token in its last page is not used, whatever it holds.
+ */
+typedef struct fkda_latent_decode_params {
+    const void *q, *cache;
+    const int32_t *block_table, *cache_lens;
+    void* out;
+    float* lse;
+    int64_t B, Tq, H, pages, page_size, max_pages;
+    int64_t q_stride[2], out_stride[2]; /* batch, row */
+    int64_t cache_stride[2];            /* page, token */
+    int64_t block_table_stride;
+    float scale;
+    int32_t reserved;
+    void* workspace; /* 256-byte aligned; fkda_latent_decode_workspace_bytes() of them */
+    size_t workspace_bytes;
+} fkda_latent_decode_params;
+size_t fkda_latent_decode_workspace_bytes(const fkda_latent_decode_params* p);
+int fkda_latent_attention_decode(const fkda_latent_decode_params* p, void* stream);
+
+/* FKDA_OK, or FKDA_ERR_DEVICE_STATUS if a kernel of the operators above gave up on a bounded wait on the current device since
+ * the last call of this function (its outputs are then not to be used).  Synchronises the stream. */
+int fkda_operator_status(void* stream);
 
 #ifdef __cplusplus
 }
