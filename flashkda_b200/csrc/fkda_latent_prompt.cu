@@ -233,6 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
         float top = -INFINITY, sum = 0.0f;
         uint32_t s[128];
         for (int i = 0; i < n[w]; ++i) {
+            if (i > 0) wait(&bar.o_done[w], (i - 1) & 1, &bar.abort);   // (issued in front of these scores)
             wait(&bar.s_full[w], i & 1, &bar.abort);
             fence_after();
 #pragma unroll
@@ -251,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
                 const float factor = move ? (top == -INFINITY ? 0.0f : ex2_approx((top - m) * c)) : 1.0f;
                 if (move) top = m;
                 sum *= factor;
-                if (i > 0) {   // (the product with the last block's values is complete: the scores were issued behind it)
+                if (i > 0) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         uint32_t o[32];

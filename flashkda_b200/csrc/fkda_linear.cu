@@ -56,7 +56,7 @@ struct Decays {
 };
 struct Bars {
     Decays decay[2];
-    uint64_t full[kStages], empty[kStages], dec_full[2], dec_empty[2], score, p_full, out_full, out_free, s_ready, s_done, split_full, drained;
+    uint64_t full[kStages], empty[kStages], dec_full[2], dec_empty[2], score[2], p_full, out_full, out_free, s_ready, s_done, split_full, drained;
     uint32_t tmem;
     int abort;
 };
@@ -135,8 +135,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) mbar_init(&bar.full[i], 1), mbar_init(&bar.empty[i], 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&bar.dec_full[i], 1), mbar_init(&bar.dec_empty[i], 12);
-        mbar_init(&bar.score, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&bar.dec_full[i], 1), mbar_init(&bar.dec_empty[i], 12), mbar_init(&bar.score[i], 1);
         mbar_init(&bar.p_full, 128);
         mbar_init(&bar.out_full, 1);
         mbar_init(&bar.out_free, 128);
@@ -193,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
                 for (int x = 0; x < 2; ++x)
                     for (int i = 0; i < 4; ++i)
                         mma_ss(tmem + kScore + (c & 1) * 64, desc(q + x * kTileBytes + i * 32), desc(k + x * kTileBytes + i * 32), kIdScore, (x | i) != 0);
-                commit(&bar.score);
+                commit(&bar.score[c & 1]);   // (one barrier per buffer: chunk c + 1's scores may be there before chunk c's outputs are away)
             };
             score(0);
             for (int c = 0; c < n && ok; ++c) {
@@ -318,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
             wait(&bar.dec_full[c & 1], (c >> 1) & 1, &bar.abort);
             const Decays& d = bar.decay[c & 1];
             const float G0 = d.G[r0], G1 = d.G[r1], e0 = d.eG[r0] * a.scale, e1 = d.eG[r1] * a.scale;
-            wait(&bar.score, c & 1, &bar.abort);
+            wait(&bar.score[c & 1], (c >> 1) & 1, &bar.abort);
             fence_after();
             uint32_t s[32], p[16];
             ld_frag64(tmem + kScore + (c & 1) * 64 + lanes, s);

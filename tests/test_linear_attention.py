@@ -177,6 +177,19 @@ def test_runs_repeat_bit_for_bit_on_two_streams_at_once(T):
 
 
 @gpu
+def test_many_long_chains_back_to_back():
+    """More chains than SMs, calls behind one another without a pause: no stage of a chunk may be passed twice by another."""
+    d = linear_inputs([2000, 900, 1, 63, 1500, 700], 48, 12, seed=13, packed=True)
+    hT = torch.zeros(6, 48, 128, 128, device="cuda")
+    call(d, h0=d["h0"], hT=hT)
+    want, state = d["out"].clone(), hT.clone()
+    for _ in range(30):
+        call(d, h0=d["h0"], hT=hT)
+    assert flashkda_b200.operator_status() == 0
+    assert torch.equal(d["out"], want) and torch.equal(hT, state)
+
+
+@gpu
 @pytest.mark.parametrize("lens", [[1, 1], [150, 150], [1, 90, 1]], ids=str)
 def test_captured_and_replayed(lens):
     packed = len(set(lens)) > 1
