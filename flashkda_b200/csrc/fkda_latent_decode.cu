@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
             float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
             const int seen[2] = {min(walk.len, walk.len - a.Tq + 1 + news[0]), min(walk.len, walk.len - a.Tq + 1 + news[1])};
             for (int t = walk.t; t < walk.until; ++t, ++g) {
-                wait(&bar.s_full[g & 1], (g >> 1) & 1, &bar.abort);
+                wait_warp(&bar.s_full[g & 1], (g >> 1) & 1, &bar.abort);
                 fence_after();
                 uint32_t s[32];
                 ld_frag64(tmem + kS + (g & 1) * kTok + lanes, s);
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
                 }
                 const bool moved = named_any(1, 128, (move[0] || move[1]) && t > walk.t);
                 if (g > 0) {   // the last value product: it has read the weights, and its outputs are there
-                    wait(&bar.o_done, (g - 1) & 1, &bar.abort);
+                    wait_warp(&bar.o_done, (g - 1) & 1, &bar.abort);
                     fence_after();
                 }
                 if (moved) {
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
                 }
             }
             named_sync(1, 128);
-            wait(&bar.o_done, (g - 1) & 1, &bar.abort);
+            wait_warp(&bar.o_done, (g - 1) & 1, &bar.abort);
             fence_after();
 #pragma unroll 1
             for (int k = 0; k < 8; ++k) {

@@ -233,8 +233,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
         float top = -INFINITY, sum = 0.0f;
         uint32_t s[128];
         for (int i = 0; i < n[w]; ++i) {
-            if (i > 0) wait(&bar.o_done[w], (i - 1) & 1, &bar.abort);   // (issued in front of these scores)
-            wait(&bar.s_full[w], i & 1, &bar.abort);
+            if (i > 0) wait_warp(&bar.o_done[w], (i - 1) & 1, &bar.abort);   // (issued in front of these scores)
+            wait_warp(&bar.s_full[w], i & 1, &bar.abort);
             fence_after();
 #pragma unroll
             for (int k = 0; k < 4; ++k) ld32(ts + k * 32, s + k * 32);
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
                 const int from = p.len_k - i * kTile;
                 for (int v = 0; v < kValueTiles; ++v) {
                     const int sl = i * (kKeyTiles + kValueTiles) + kKeyTiles + v;
-                    wait(&bar.full[sl % kSlots], (sl / kSlots) & 1, &bar.abort);
+                    wait_warp(&bar.full[sl % kSlots], (sl / kSlots) & 1, &bar.abort);
                     uint4* dst = reinterpret_cast<uint4*>(ring + (sl % kSlots) * kSlotBytes);
                     for (int k = from * 8 + (threadIdx.x & 127); k < kTile * 8; k += 128) dst[k] = make_uint4(0, 0, 0, 0);
                 }
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
             arrive(&bar.p_full[w]);
         }
         if (n[w] > 0) {
-            wait(&bar.o_done[w], (n[w] - 1) & 1, &bar.abort);
+            wait_warp(&bar.o_done[w], (n[w] - 1) & 1, &bar.abort);
             fence_after();
         }
         const bool mine = p.any && row < p.len_q;

@@ -26,14 +26,14 @@ constexpr int kC = 64;                        // tokens of a chunk
 constexpr int kTileBytes = kC * 128;          // 64 tokens x 64 dimensions
 constexpr int kOperandBytes = 2 * kTileBytes; // a chunk of q, k or v
 constexpr int kStageBytes = 3 * kOperandBytes;
-constexpr int kStages = 2;
+constexpr int kStages = 3;
 constexpr int kTerms = 3;
-constexpr int kThreads = 480;
-constexpr int kOffSplit = kStages * kStageBytes;
-constexpr int kOffState = kOffSplit + kTerms * kOperandBytes;
-constexpr int kOffOut = kOffState + kD * kD * 2;
-constexpr int kOffBars = kOffOut + kC * kD * 2;
-constexpr uint32_t kS = 0, kScore = 128, kO1 = 256, kO2 = 384;   // tensor-memory columns
+constexpr int kThreads = 896;                 // warpgroups: one each for state and scores, two each for outputs and values; copies, products, decays
+constexpr int kOffP = kStages * kStageBytes;
+constexpr int kOffOut = kOffP + 2 * kTileBytes;
+constexpr int kOffBars = kOffOut + 2 * kOperandBytes;
+// Tensor-memory columns: the state, its bf16 copy, scores, the two parts of the outputs, the weighted values' terms
+constexpr uint32_t kS = 0, kCopy = 128, kScore = 192, kO1 = 256, kO2 = 320, kW = 384;
 
 struct LinearArgs {
     const float* g;
@@ -48,15 +48,17 @@ struct LinearArgs {
     bool state_fp32, skip_single;
 };
 struct LinearMaps {
-    CUtensorMap q, k, v;
+    CUtensorMap q, k, v, out;
 };
 struct Decays {
     float G[kC], eG[kC], w[kC], total;
     float pad[3];
 };
+// (A barrier that one side may complete twice before the other has looked is there once per buffer.)
 struct Bars {
-    Decays decay[2];
-    uint64_t full[kStages], empty[kStages], dec_full[2], dec_empty[2], score[2], p_full, out_full, out_free, s_ready, s_done, split_full, drained;
+    Decays decay[kStages];
+    uint64_t full[kStages], empty[kStages], dec_full[kStages], dec_empty[kStages], score, score_free, p_full[2], p_free[2], out_full, out_free, scaled[2], s_done[2], copy_free,
+        w_full[2], drained[2];
     uint32_t tmem;
     int abort;
 };
@@ -134,19 +136,19 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     Bars& bar = *reinterpret_cast<Bars*>(smem + kOffBars);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kStages; ++i) mbar_init(&bar.full[i], 1), mbar_init(&bar.empty[i], 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&bar.dec_full[i], 1), mbar_init(&bar.dec_empty[i], 12), mbar_init(&bar.score[i], 1);
-        mbar_init(&bar.p_full, 128);
+        for (int i = 0; i < kStages; ++i) mbar_init(&bar.full[i], 1), mbar_init(&bar.empty[i], 2), mbar_init(&bar.dec_full[i], 1), mbar_init(&bar.dec_empty[i], 24);
+        for (int i = 0; i < 2; ++i) mbar_init(&bar.p_full[i], 128), mbar_init(&bar.p_free[i], 1), mbar_init(&bar.w_full[i], 128);
+        mbar_init(&bar.score, 1);
+        mbar_init(&bar.score_free, 128);
         mbar_init(&bar.out_full, 1);
-        mbar_init(&bar.out_free, 128);
-        mbar_init(&bar.s_ready, 128);
-        mbar_init(&bar.s_done, 1);
-        mbar_init(&bar.split_full, 128);
-        mbar_init(&bar.drained, 1);
+        mbar_init(&bar.out_free, 256);
+        for (int i = 0; i < 2; ++i) mbar_init(&bar.scaled[i], 128), mbar_init(&bar.s_done[i], 1);
+        mbar_init(&bar.copy_free, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&bar.drained[i], 1);
         bar.abort = 0;
         mbar_fence_init();
     }
-    if (warp == 13) tmem_alloc(&bar.tmem, 512);
+    if (warp == 25) tmem_alloc(&bar.tmem, 512);
     fence_before();
     grid_dep_launch();
     grid_dep_wait();
@@ -157,11 +159,12 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     const bool mine = !(a.skip_single && ch.len <= 1);
     const int n = mine ? (ch.len + kC - 1) / kC : 0;
 
-    if (warp == 12) {
+    if (warp == 24) {
         // ---- copies ----
         if (elect_one()) {
             bool ok = true;
             int c = 0;
+#pragma unroll 1
             for (; c < n; ++c) {
                 const int s = c % kStages;
                 if (c >= kStages) ok = wait(&bar.empty[s], (c / kStages - 1) & 1, &bar.abort);
@@ -177,55 +180,85 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
             }
             for (int k = max(0, c - kStages); k < c; ++k) drain(&bar.full[k % kStages], (k / kStages) & 1);
         }
-    } else if (warp == 13) {
-        // ---- products ----
+    } else if (warp == 25) {
+        // ---- products of the state, which the next chunk waits for, and scores ----
         if (n > 0 && elect_one()) {
-            const uint32_t base = smem_u32(smem), split = base + kOffSplit, state = base + kOffState;
-            constexpr uint32_t kIdScore = idesc(64, 64, false, false), kIdOut1 = idesc(64, 128, false, false),
-                               kIdOut2 = idesc(64, 128, false, true), kIdState = idesc(128, 128, true, true);
+            const uint32_t base = smem_u32(smem);
+            constexpr uint32_t kIdScore = idesc(64, 64, false, false), kIdState = idesc(128, 64, false, true);
             bool ok = true;
+            auto until = [&](uint64_t* b, int phase) { ok = ok && wait(b, phase & 1, &bar.abort); };
             auto score = [&](int c) {
-                ok = wait(&bar.full[c % kStages], (c / kStages) & 1, &bar.abort);
+                until(&bar.full[c % kStages], c / kStages);
+                if (c > 0) until(&bar.score_free, c - 1);
                 if (!ok) return;
                 fence_after();
                 const uint32_t q = base + (c % kStages) * kStageBytes, k = q + kOperandBytes;
                 for (int x = 0; x < 2; ++x)
                     for (int i = 0; i < 4; ++i)
-                        mma_ss(tmem + kScore + (c & 1) * 64, desc(q + x * kTileBytes + i * 32), desc(k + x * kTileBytes + i * 32), kIdScore, (x | i) != 0);
-                commit(&bar.score[c & 1]);   // (one barrier per buffer: chunk c + 1's scores may be there before chunk c's outputs are away)
+                        mma_ss(tmem + kScore, desc(q + x * kTileBytes + i * 32), desc(k + x * kTileBytes + i * 32), kIdScore, (x | i) != 0);
+                commit(&bar.score);
             };
             score(0);
+#pragma unroll 1
             for (int c = 0; c < n && ok; ++c) {
-                const uint32_t q = base + (c % kStages) * kStageBytes, k = q + kOperandBytes, v = k + kOperandBytes;
-                ok = wait(&bar.s_ready, c & 1, &bar.abort) && (c == 0 || wait(&bar.out_free, (c - 1) & 1, &bar.abort));
+                const uint32_t k = base + (c % kStages) * kStageBytes + kOperandBytes;
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {   // 64 columns of the state, while the other 64 are being decayed
+                    until(&bar.scaled[h], c);
+                    for (int half = 0; half < 2; ++half) {
+                        if (h == 0) until(&bar.w_full[half], c);
+                        if (!ok) break;
+                        fence_after();
+                        for (int i = 2 * half; i < 2 * half + 2; ++i)
+                            for (int t = 0; t < kTerms; ++t)
+                                mma_ts(tmem + kS + h * 64, tmem + kW + t * 32 + i * 8, desc(k + h * kTileBytes + i * 2048), kIdState, 1);
+                    }
+                    if (!ok) break;
+                    commit(&bar.s_done[h]);
+                }
+                if (!ok) break;
+                commit(&bar.empty[c % kStages]);
+                if (c + 1 < n) score(c + 1);
+            }
+            commit(&bar.drained[0]);
+            drain(&bar.drained[0], 0);
+        }
+    } else if (warp == 27) {
+        // ---- products of the outputs ----
+        if (n > 0 && elect_one()) {
+            const uint32_t base = smem_u32(smem), p_addr = base + kOffP;
+            constexpr uint32_t kIdO1 = idesc(128, 64, false, false), kIdO2 = idesc(128, 64, true, false);
+            bool ok = true;
+            auto until = [&](uint64_t* b, int phase) { ok = ok && wait(b, phase & 1, &bar.abort); };
+#pragma unroll 1
+            for (int c = 0; c < n; ++c) {
+                const uint32_t q = base + (c % kStages) * kStageBytes, v = q + 2 * kOperandBytes;
+                until(&bar.full[c % kStages], c / kStages);
+                until(&bar.scaled[1], c);   // (the copy is there as well)
+                if (c > 0) until(&bar.out_free, c - 1);
                 if (!ok) break;
                 fence_after();
                 for (int x = 0; x < 2; ++x)
                     for (int i = 0; i < 4; ++i)
-                        mma_ss(tmem + kO1, desc(q + x * kTileBytes + i * 32), desc(state + x * (kD * 128) + i * 32), kIdOut1, (x | i) != 0);
-                ok = wait(&bar.split_full, c & 1, &bar.abort);
-                if (!ok) break;
-                fence_after();
-                for (int t = 0; t < kTerms; ++t)
-                    for (int i = 0; i < 4; ++i)
-                        mma_ss(tmem + kS, desc(split + t * kOperandBytes + i * 2048, kTileBytes), desc(k + i * 2048, kTileBytes), kIdState, 1);
-                commit(&bar.s_done);
-                if (c + 1 < n) score(c + 1);
-                if (!ok) break;
-                ok = wait(&bar.p_full, c & 1, &bar.abort);
+                        mma_ts(tmem + kO1, tmem + kCopy + x * 32 + i * 8, desc(q + x * kTileBytes + i * 32), kIdO1, (x | i) != 0);
+                commit(&bar.copy_free);
+                if (c + 1 == n) until(&bar.w_full[1], c);   // (values behind the sequence's end are nothing by now)
+                until(&bar.p_full[c & 1], c >> 1);
                 if (!ok) break;
                 fence_after();
                 for (int i = 0; i < 4; ++i)
-                    mma_ts(tmem + kO2, tmem + kScore + (c & 1) * 64 + i * 8, desc(v + i * 2048, kTileBytes), kIdOut2, i != 0);
+                    mma_ss(tmem + kO2, desc(v + i * 2048, kTileBytes), desc(p_addr + (c & 1) * kTileBytes + i * 32), kIdO2, i != 0);
+                commit(&bar.p_free[c & 1]);
                 commit(&bar.out_full);
                 commit(&bar.empty[c % kStages]);
             }
-            commit(&bar.drained);
-            drain(&bar.drained, 0);
+            commit(&bar.drained[1]);
+            drain(&bar.drained[1], 0);
         }
-    } else if (warp == 14) {
+    } else if (warp == 26) {
         // ---- decays: lane l has tokens 2 l and 2 l + 1 of a chunk ----
         const float* g = a.g + ch.b * a.g_batch + ch.t0 * a.g_token + ch.h * a.g_head;
+#pragma unroll 1
         for (int c = 0; c < n; ++c) {
             const int t = c * kC + 2 * lane;
             const float x = t < ch.len ? log2_decay(g[t * a.g_token]) : 0.0f, y = t + 1 < ch.len ? log2_decay(g[(t + 1) * a.g_token]) : 0.0f;
@@ -238,62 +271,68 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
             }
             const float before = __shfl_up_sync(0xffffffffu, upto, 1), behind = __shfl_down_sync(0xffffffffu, from, 1);
             const float G0 = (lane > 0 ? before : 0.0f) + x, G1 = G0 + y, w1 = lane < 31 ? behind : 0.0f, w0 = w1 + y;
-            if (c >= 2) wait(&bar.dec_empty[c & 1], (c / 2 - 1) & 1, &bar.abort);
-            Decays& d = bar.decay[c & 1];
-            d.G[2 * lane] = G0;
-            d.G[2 * lane + 1] = G1;
-            d.eG[2 * lane] = ex2_approx(G0);
-            d.eG[2 * lane + 1] = ex2_approx(G1);
-            d.w[2 * lane] = ex2_approx(w0);
-            d.w[2 * lane + 1] = ex2_approx(w1);
+            if (c >= kStages) wait_warp(&bar.dec_empty[c % kStages], (c / kStages - 1) & 1, &bar.abort);
+            Decays& d = bar.decay[c % kStages];
+            *reinterpret_cast<float2*>(&d.G[2 * lane]) = make_float2(G0, G1);
+            *reinterpret_cast<float2*>(&d.eG[2 * lane]) = make_float2(ex2_approx(G0) * a.scale, ex2_approx(G1) * a.scale);
+            *reinterpret_cast<float2*>(&d.w[2 * lane]) = make_float2(ex2_approx(w0), ex2_approx(w1));
             if (lane == 0) d.total = ex2_approx(from);
             __syncwarp();
-            if (lane == 0) arrive(&bar.dec_full[c & 1]);
+            if (lane == 0) arrive(&bar.dec_full[c % kStages]);
         }
     } else if (warp < 4) {
-        // ---- state: thread = row ----
+        // ---- state: thread = row (dimension of v); decayed in place, with a bf16 copy of what it was for the product with q ----
         const int v = warp * 32 + lane;
-        const uint32_t ts = tmem + kS + ((uint32_t)(warp * 32) << 16);
+        const uint32_t lanes = (uint32_t)(warp * 32) << 16, ts = tmem + kS + lanes;
         const int64_t at = ((ch.n * a.H + ch.h) * kD + v) * (int64_t)kD;
-        uint8_t* row = smem + kOffState + v * 128;
-        for (int c = 0; c < n; ++c) {
-            wait(&bar.dec_full[c & 1], (c >> 1) & 1, &bar.abort);
-            const float total = bar.decay[c & 1].total;
-            __syncwarp();
-            mbar_arrive_lane0(&bar.dec_empty[c & 1], lane);
-            if (c > 0) {
-                wait(&bar.s_done, (c - 1) & 1, &bar.abort);
-                fence_after();
-            }
-#pragma unroll
+        if (n > 0) {
+#pragma unroll 1
             for (int x = 0; x < 4; ++x) {
                 uint32_t r[32];
-                if (c > 0) {
-                    ld32(ts + x * 32, r);
-                    wait_ld();
-                } else {
-                    load_state32(a, at + x * 32, r);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<uint4*>(row + (x >> 1) * (kD * 128) + ((((x & 1) * 4 + i) ^ (v & 7)) << 4)) =
-                        make_uint4(pack_bf2(f(r[8 * i]), f(r[8 * i + 1])), pack_bf2(f(r[8 * i + 2]), f(r[8 * i + 3])),
-                                   pack_bf2(f(r[8 * i + 4]), f(r[8 * i + 5])), pack_bf2(f(r[8 * i + 6]), f(r[8 * i + 7])));
-#pragma unroll
-                for (int i = 0; i < 32; ++i) r[i] = u(f(r[i]) * total);
+                load_state32(a, at + x * 32, r);
                 st32(ts + x * 32, r);
             }
             wait_st();
-            fence_proxy_async_smem();
-            fence_before();
-            arrive(&bar.s_ready);
+        }
+#pragma unroll 1
+        for (int c = 0; c < n; ++c) {
+            const int s = c % kStages;
+            wait_warp(&bar.dec_full[s], (c / kStages) & 1, &bar.abort);
+            const float total = bar.decay[s].total;
+            __syncwarp();
+            mbar_arrive_lane0(&bar.dec_empty[s], lane);
+            if (c > 0) wait_warp(&bar.copy_free, (c - 1) & 1, &bar.abort);
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+                if (c > 0) {
+                    wait_warp(&bar.s_done[h], (c - 1) & 1, &bar.abort);
+                    fence_after();
+                }
+#pragma unroll 1
+                for (int x = 2 * h; x < 2 * h + 2; ++x) {
+                    uint32_t r[32], copy[16];
+                    ld32(ts + x * 32, r);
+                    wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        copy[i] = pack_bf2(f(r[2 * i]), f(r[2 * i + 1]));
+                        mul2(r[2 * i], r[2 * i + 1], total, total);
+                    }
+                    st32(ts + x * 32, r);
+                    st16(tmem + kCopy + lanes + x * 16, copy);
+                }
+                wait_st();
+                fence_before();
+                arrive(&bar.scaled[h]);
+            }
         }
         if (n > 0) {
-            wait(&bar.s_done, (n - 1) & 1, &bar.abort);
+            wait_warp(&bar.s_done[0], (n - 1) & 1, &bar.abort);
+            wait_warp(&bar.s_done[1], (n - 1) & 1, &bar.abort);
             fence_after();
         }
         if (mine && a.hT != nullptr) {
-#pragma unroll
+#pragma unroll 1
             for (int x = 0; x < 4; ++x) {
                 uint32_t r[32];
                 if (n > 0) {
@@ -307,115 +346,175 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         }
         fence_before();
     } else if (warp < 8) {
-        // ---- scores to weights, outputs: warp w has rows 16 w .. 16 w + 15, thread 4 g + t rows g and g + 8 of these ----
+        // ---- scores to weights: warp w has rows (queries) 16 w .. 16 w + 15, thread 4 g + t rows g and g + 8 of these ----
         const int w = warp - 4, gr = lane >> 2, tc = lane & 3;
         const int r0 = w * 16 + gr, r1 = r0 + 8;
-        const uint32_t lanes = (uint32_t)(w * 32) << 16;
-        uint8_t* stage = smem + kOffOut + w * 16 * 256;
-        __nv_bfloat16* out = a.out + ch.b * a.out_batch + ch.t0 * a.out_token + ch.h * a.out_head;
+#pragma unroll 1
         for (int c = 0; c < n; ++c) {
-            wait(&bar.dec_full[c & 1], (c >> 1) & 1, &bar.abort);
-            const Decays& d = bar.decay[c & 1];
-            const float G0 = d.G[r0], G1 = d.G[r1], e0 = d.eG[r0] * a.scale, e1 = d.eG[r1] * a.scale;
-            wait(&bar.score[c & 1], (c >> 1) & 1, &bar.abort);
+            wait_warp(&bar.dec_full[c % kStages], (c / kStages) & 1, &bar.abort);
+            const Decays& d = bar.decay[c % kStages];
+            const float G0 = d.G[r0], G1 = d.G[r1];
+            if (c >= 2) wait_warp(&bar.p_free[c & 1], (c / 2 - 1) & 1, &bar.abort);
+            wait_warp(&bar.score, c & 1, &bar.abort);
             fence_after();
-            uint32_t s[32], p[16];
-            ld_frag64(tmem + kScore + (c & 1) * 64 + lanes, s);
-            wait_ld();
+            uint8_t* p = smem + kOffP + (c & 1) * kTileBytes + r0 * 128 + tc * 4;   // (r1 = r0 + 8 has the same swizzle)
+#pragma unroll 1
+            for (int b = 0; b < 4; ++b) {   // 16 columns; those behind the warp's last row are masked for all of its rows
+                uint32_t s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                if (b <= w) {
+                    ld_frag16(tmem + kScore + b * 16 + ((uint32_t)(w * 32) << 16), s);
+                    wait_ld();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (i <= 2 * w + 1) {   // (columns behind the warp's last row are masked for all of its rows)
-                    const int j = 8 * i + 2 * tc;
-                    const float2 G = *reinterpret_cast<const float2*>(&d.G[j]);
-                    const float a0 = j <= r0 ? f(s[4 * i]) * ex2_approx(G0 - G.x) : 0.0f, a1 = j + 1 <= r0 ? f(s[4 * i + 1]) * ex2_approx(G0 - G.y) : 0.0f;
-                    const float b0 = j <= r1 ? f(s[4 * i + 2]) * ex2_approx(G1 - G.x) : 0.0f, b1 = j + 1 <= r1 ? f(s[4 * i + 3]) * ex2_approx(G1 - G.y) : 0.0f;
-                    p[2 * i] = pack_bf2(a0, a1);
-                    p[2 * i + 1] = pack_bf2(b0, b1);
-                } else {
-                    p[2 * i] = p[2 * i + 1] = 0u;
+                    for (int i = 0; i < 2; ++i) {
+                        const int j = b * 16 + 8 * i + 2 * tc;
+                        const float2 G = *reinterpret_cast<const float2*>(&d.G[j]);
+                        s[4 * i] = j <= r0 ? u(f(s[4 * i]) * ex2_approx(G0 - G.x)) : 0u;
+                        s[4 * i + 1] = j < r0 ? u(f(s[4 * i + 1]) * ex2_approx(G0 - G.y)) : 0u;
+                        s[4 * i + 2] = j <= r1 ? u(f(s[4 * i + 2]) * ex2_approx(G1 - G.x)) : 0u;
+                        s[4 * i + 3] = j < r1 ? u(f(s[4 * i + 3]) * ex2_approx(G1 - G.y)) : 0u;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int unit = ((2 * b + i) ^ gr) << 4;
+                    *reinterpret_cast<uint32_t*>(p + unit) = pack_bf2(f(s[4 * i]), f(s[4 * i + 1]));
+                    *reinterpret_cast<uint32_t*>(p + 8 * 128 + unit) = pack_bf2(f(s[4 * i + 2]), f(s[4 * i + 3]));
                 }
             }
-            st_frag32(tmem + kScore + (c & 1) * 64 + lanes, p);
-            wait_st();
             fence_before();
-            arrive(&bar.p_full);
+            arrive(&bar.score_free);
+            fence_proxy_async_smem();
+            arrive(&bar.p_full[c & 1]);
             __syncwarp();
-            mbar_arrive_lane0(&bar.dec_empty[c & 1], lane);
-
-            wait(&bar.out_full, c & 1, &bar.abort);
+            mbar_arrive_lane0(&bar.dec_empty[c % kStages], lane);
+        }
+    } else if (warp < 16) {
+        // ---- outputs: fragments of 16 dimensions of v x 32 tokens, stored transposed as rows of tokens, which one copy takes away (or the
+        //      warps themselves, where the chunk's last rows are not the sequence's) ----
+        const int w = warp & 3, half = (warp - 8) >> 2, tc = lane & 3, me = threadIdx.x & 255;   // a warpgroup has 32 of the tokens
+        // the lane's row address within four 8 x 8 blocks (two of tokens x two of dimensions)
+        const int token = (lane & 7) + ((lane >> 4) << 3), unit = (w & 1) * 4 + ((lane >> 3) & 1);
+        const uint32_t tile = smem_u32(smem) + kOffOut + (w >> 1) * kTileBytes + token * 128;
+#pragma unroll 1
+        for (int c = 0; c < n; ++c) {
+            const Decays& d = bar.decay[c % kStages];
+            const uint32_t buffer = tile + (c & 1) * kOperandBytes;
+            const int valid = ch.len - c * kC;
+            if (me == 0) bulk_wait_group_read<1>();   // (the copy that the buffer's last outputs went with)
+            wait_warp(&bar.dec_full[c % kStages], (c / kStages) & 1, &bar.abort);
+            named_sync(2, 256);
+            wait_warp(&bar.out_full, c & 1, &bar.abort);
             fence_after();
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                uint32_t o1[32], o2[32];
-                ld_frag64(tmem + kO1 + x * 64 + lanes, o1);
-                ld_frag64(tmem + kO2 + x * 64 + lanes, o2);
+#pragma unroll 1
+            for (int up = 0; up < 2; ++up) {   // 16 of the warp's dimensions
+                const uint32_t lanes = (uint32_t)(w * 32 + up * 16) << 16;
+                uint32_t o1[16], o2[16];
+                ld_frag32(tmem + kO1 + half * 32 + lanes, o1);
+                ld_frag32(tmem + kO2 + half * 32 + lanes, o2);
                 wait_ld();
+                const uint32_t row = buffer + half * 32 * 128 + (((unit + 2 * up) ^ (lane & 7)) << 4);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int unit = (x * 8 + i) ^ gr;
-                    *reinterpret_cast<uint32_t*>(stage + gr * 256 + unit * 16 + tc * 4) =
-                        pack_bf2(__fmaf_rn(f(o1[4 * i]), e0, f(o2[4 * i]) * a.scale), __fmaf_rn(f(o1[4 * i + 1]), e0, f(o2[4 * i + 1]) * a.scale));
-                    *reinterpret_cast<uint32_t*>(stage + (gr + 8) * 256 + unit * 16 + tc * 4) =
-                        pack_bf2(__fmaf_rn(f(o1[4 * i + 2]), e1, f(o2[4 * i + 2]) * a.scale), __fmaf_rn(f(o1[4 * i + 3]), e1, f(o2[4 * i + 3]) * a.scale));
+                for (int i = 0; i < 2; ++i) {   // 16 tokens
+                    uint32_t y[4];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float2 e = *reinterpret_cast<const float2*>(&d.eG[half * 32 + i * 16 + j * 8 + 2 * tc]);
+                        const uint32_t *p1 = o1 + 8 * i + 4 * j, *p2 = o2 + 8 * i + 4 * j;
+                        y[2 * j] = pack_bf2(__fmaf_rn(f(p1[0]), e.x, f(p2[0]) * a.scale), __fmaf_rn(f(p1[1]), e.y, f(p2[1]) * a.scale));
+                        y[2 * j + 1] = pack_bf2(__fmaf_rn(f(p1[2]), e.x, f(p2[2]) * a.scale), __fmaf_rn(f(p1[3]), e.y, f(p2[3]) * a.scale));
+                    }
+                    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(row + i * 16 * 128), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
                 }
             }
             fence_before();
             arrive(&bar.out_free);
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = 2 * i + (lane >> 4), t = c * kC + w * 16 + r;
-                const uint4 x = *reinterpret_cast<const uint4*>(stage + r * 256 + (((lane & 15) ^ (r & 7)) << 4));
-                if (t < ch.len) *reinterpret_cast<uint4*>(out + t * a.out_token + (lane & 15) * 8) = x;
-            }
-            __syncwarp();
-        }
-    } else {
-        // ---- weighted values in three terms; rows behind the sequence's end become nothing ----
-        const int me = (warp - 8) * 32 + lane;
-        for (int c = 0; c < n; ++c) {
-            const int s = c % kStages, valid = min(kC, ch.len - c * kC);
-            uint8_t* k = smem + s * kStageBytes + kOperandBytes;
-            uint8_t* v = k + kOperandBytes;
-            uint8_t* split = smem + kOffSplit;
-            wait(&bar.dec_full[c & 1], (c >> 1) & 1, &bar.abort);
-            float w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = bar.decay[c & 1].w[i * 16 + (me >> 3)];
-            __syncwarp();
-            mbar_arrive_lane0(&bar.dec_empty[c & 1], lane);
-            wait(&bar.full[s], (c / kStages) & 1, &bar.abort);
-            if (c > 0) wait(&bar.s_done, (c - 1) & 1, &bar.abort);   // (the last chunk's terms have been read)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int at = (i * 128 + me) * 16, t = (i & 3) * 16 + (me >> 3);   // 16 bytes of token t
-                uint4 x = *reinterpret_cast<const uint4*>(v + at);
-                if (t >= valid) {
-                    x = make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4*>(v + at) = x;
-                    *reinterpret_cast<uint4*>(k + at) = x;
+            fence_proxy_async_smem();
+            named_sync(2, 256);
+            mbar_arrive_lane0(&bar.dec_empty[c % kStages], lane);
+            if (valid >= kC) {
+                if (me == 0) {
+                    const uint8_t* src = smem + kOffOut + (c & 1) * kOperandBytes;
+                    for (int x = 0; x < 2; ++x) tma_store_4d(&maps.out, x * 64, ch.h, (int)ch.t0 + c * kC, (int)ch.b, src + x * kTileBytes);
+                    bulk_commit_group();
                 }
-                uint32_t in[4] = {x.x, x.y, x.z, x.w}, term[kTerms][4];
+            } else {
+                __nv_bfloat16* out = a.out + ch.b * a.out_batch + (ch.t0 + c * kC) * a.out_token + ch.h * a.out_head;
+#pragma unroll 1
+                for (int i = me; i < valid * 16; i += 256) {
+                    const int t = i >> 4, x = i & 15;
+                    *reinterpret_cast<uint4*>(out + t * a.out_token + x * 8) =
+                        *reinterpret_cast<const uint4*>(smem + kOffOut + (c & 1) * kOperandBytes + (x >> 3) * kTileBytes + t * 128 + (((x ^ t) & 7) << 4));
+                }
+            }
+        }
+        if (me == 0) bulk_wait_group<0>();
+    } else {
+        // ---- weighted values: transposed reads give thread 4 g + t of warp w the token pairs 8 b + 2 t, + 1 of dimensions g, g + 8, g + 16
+        //      and g + 24 of the warp's 32, as the A operand wants them; what is behind the sequence's end becomes nothing ----
+        const int w = warp & 3, half = (warp - 16) >> 2, tc = lane & 3;   // a warpgroup has 32 of the tokens
+        // the lane's row address within a group of four 8 x 8 blocks (two of tokens x two of dimensions)
+        const int token = (lane & 7) + ((lane >> 4) << 3);            // of 16
+        const int unit = (w & 1) * 4 + ((lane >> 3) & 1);               // 16-byte piece of the tile's row, + 2 for the upper 16 dimensions
+        const uint32_t tile = smem_u32(smem) + 2 * kOperandBytes + (w >> 1) * kTileBytes + token * 128;
+        const uint32_t piece[2] = {tile + ((unit ^ (lane & 7)) << 4), tile + (((unit + 2) ^ (lane & 7)) << 4)};
+        const uint32_t tw = tmem + kW + ((uint32_t)(w * 32) << 16);
+#pragma unroll 1
+        for (int c = 0; c < n; ++c) {
+            const int s = c % kStages, valid = ch.len - c * kC;
+            wait_warp(&bar.dec_full[s], (c / kStages) & 1, &bar.abort);
+            wait_warp(&bar.full[s], (c / kStages) & 1, &bar.abort);
+            if (valid < kC) {
+                uint8_t* k = smem + s * kStageBytes + kOperandBytes;
+#pragma unroll 1
+                for (int i = threadIdx.x & 255; i < (kC - valid) * 8; i += 256)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float lo = bf_lo(in[j]) * w[i & 3], hi = bf_hi(in[j]) * w[i & 3];
+                    for (int x = 0; x < 4; ++x) *reinterpret_cast<uint4*>(k + x * kTileBytes + valid * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+                fence_proxy_async_smem();
+                named_sync(1, 256);
+            }
+            uint32_t term[2][2][kTerms][4];
 #pragma unroll
-                    for (int m = 0; m < kTerms; ++m) {
-                        term[m][j] = pack_bf2(lo, hi);
-                        lo -= bf_lo(term[m][j]);
-                        hi -= bf_hi(term[m][j]);
+            for (int b = 0; b < 2; ++b) {          // 16 tokens
+                const float *w0 = &bar.decay[s].w[half * 32 + b * 16 + 2 * tc], *w1 = w0 + 8;
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {      // 16 dimensions
+                    uint32_t r[4];
+                    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(piece[d] + s * kStageBytes + (2 * half + b) * 2048) : "memory");
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {   // r[0], r[1]: tokens 0 .. 7, dimensions 0 .. 7 and 8 .. 15; r[2], r[3]: tokens 8 .. 15
+                        uint32_t x = r[i] << 16, y = r[i] & 0xffff0000u;
+                        mul2(x, y, i < 2 ? w0[0] : w1[0], i < 2 ? w0[1] : w1[1]);
+#pragma unroll
+                        for (int m = 0; m < kTerms; ++m) {
+                            // the upper 16 bits of what is left, which are a bf16: after three times nothing is
+                            term[b][d][m][i] = __byte_perm(x, y, 0x7632);
+                            if (m + 1 < kTerms) sub2(x, y, x & 0xffff0000u, y & 0xffff0000u);
+                        }
                     }
                 }
-#pragma unroll
-                for (int m = 0; m < kTerms; ++m) *reinterpret_cast<uint4*>(split + m * kOperandBytes + at) = make_uint4(term[m][0], term[m][1], term[m][2], term[m][3]);
             }
-            fence_proxy_async_smem();
-            arrive(&bar.split_full);
+            if (c > 0) {
+                wait_warp(&bar.s_done[1], (c - 1) & 1, &bar.abort);   // (the last chunk's terms have been read)
+                fence_after();
+            }
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int d = 0; d < 2; ++d)
+#pragma unroll
+                    for (int m = 0; m < kTerms; ++m)
+                        st_frag8(tw + m * 32 + (2 * half + b) * 8 + ((uint32_t)(d * 16) << 16), term[b][d][m][0], term[b][d][m][1], term[b][d][m][2], term[b][d][m][3]);
+            wait_st();
+            fence_before();
+            arrive(&bar.w_full[half]);
+            __syncwarp();
+            mbar_arrive_lane0(&bar.dec_empty[s], lane);
         }
     }
     __syncthreads();
     fence_after();
-    if (warp == 13) tmem_dealloc(tmem, 512);
+    if (warp == 25) tmem_dealloc(tmem, 512);
 }
 
 // ---- single tokens: four CTAs per chain, a warp owns eight rows of the state, lane l columns 4 l .. 4 l + 3 of each ----
@@ -534,7 +633,8 @@ int launch_linear(const fkda_linear_params& p, cudaStream_t stream, int* n_launc
             const cuuint32_t box[4] = {64u, 1u, (cuuint32_t)kC, 1u};
             return encode_bf16_map(m, 4, base, dims, strides, box);
         };
-        if (!map4(&maps.q, p.q, p.Hk, p.q_stride) || !map4(&maps.k, p.k, p.Hk, p.k_stride) || !map4(&maps.v, p.v, p.H, p.v_stride))
+        if (!map4(&maps.q, p.q, p.Hk, p.q_stride) || !map4(&maps.k, p.k, p.Hk, p.k_stride) || !map4(&maps.v, p.v, p.H, p.v_stride) ||
+            !map4(&maps.out, p.out, p.H, p.out_stride))
             return FKDA_ERR_LAUNCH;
         if (!allow_smem<linear_chunk_kernel>(kSmem)) return FKDA_ERR_LAUNCH;
         if (!launch_dependent(linear_chunk_kernel, chains, kThreads, kSmem, stream, a, maps)) return FKDA_ERR_LAUNCH;

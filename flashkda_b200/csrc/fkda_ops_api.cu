@@ -52,7 +52,7 @@ int check(fkda_linear_params* p) {
         !aligned(p->final_state, 16))
         return FKDA_ERR_ALIGNMENT;
     if (!tile_strides(p->q_stride, {p->B, p->T, p->Hk}) || !tile_strides(p->k_stride, {p->B, p->T, p->Hk}) || !tile_strides(p->v_stride, {p->B, p->T, p->H}) ||
-        !row_strides(p->out_stride, {p->B, p->T, p->H}))
+        !tile_strides(p->out_stride, {p->B, p->T, p->H}))
         return FKDA_ERR_ALIGNMENT;
     return FKDA_OK;
 }

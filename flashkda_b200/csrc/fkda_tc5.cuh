@@ -16,7 +16,21 @@ using namespace sm100;
 // return at once: the roles run to their ends on whatever is in shared memory (all accesses in bounds), the copies and
 // products in flight are waited for, tensor memory is freed, and the word below tells the host (fkda_operator_status).
 static __device__ int32_t g_gave_up = 0;
-constexpr uint64_t kWaitNs = 2000000000ull;
+// The limit is counted in SM cycles (two seconds at 2 GHz): the global timer is far away, and reading it in the waits of a dozen
+// warps made all of them slower.
+constexpr long long kWaitCycles = 4000000000ll;
+
+__device__ __forceinline__ bool wait_until(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    long long start = 0;
+    for (uint32_t spins = 0; !mbar_try_wait(bar, parity); ++spins) {
+        if ((spins & 31u) != 31u) continue;
+        if (abort_flag != nullptr && *abort_flag != 0) return false;
+        const long long now = clock64();
+        if (start == 0) start = now;
+        if (now - start > kWaitCycles) return false;
+    }
+    return true;
+}
 
 // The word of this translation unit's kernels, once the stream has come this far; cleared for the next reader.
 static int read_gave_up(cudaStream_t stream, int32_t* word) {
@@ -29,13 +43,20 @@ static int read_gave_up(cudaStream_t stream, int32_t* word) {
 }
 
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* abort_flag) {
-    if (mbar_wait_bounded(bar, parity, abort_flag, kWaitNs)) return true;
+    if (wait_until(bar, parity, abort_flag)) return true;
     *reinterpret_cast<volatile int*>(abort_flag) = 1;
     g_gave_up = 1;
     return false;
 }
+// The same for a whole warp, whose lanes leave it together: what follows may be an access to tensor memory or another instruction that
+// a warp executes as one.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* abort_flag) {
+    const bool ok = wait(bar, parity, abort_flag);
+    __syncwarp();
+    return ok;
+}
 // For what is in flight when a role ends: not cut short by the abort flag.
-__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) { mbar_wait_bounded(bar, parity, nullptr, kWaitNs); }
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) { wait_until(bar, parity, nullptr); }
 
 __device__ __forceinline__ void arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -59,6 +80,12 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* tmap, in
         "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
         ::"r"(smem_u32(smem_dst)), "l"(tmap), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
         : "memory");
+}
+
+__device__ __forceinline__ void tma_store_4d(const void* tmap, int c0, int c1, int c2, int c3, const void* smem_src) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(tmap), "r"(c0), "r"(c1), "r"(c2),
+                 "r"(c3), "r"(smem_u32(smem_src))
+                 : "memory");
 }
 
 // ---------------------------------------------------------- tensor memory ----
@@ -100,11 +127,32 @@ __device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* r) {
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
-// Fragment-shaped accesses for accumulators of 64 rows, whose rows 16 w .. 16 w + 15 live in lanes 32 w .. 32 w + 15.  Thread
-// 4 g + t of warp w:
-//   load of 64 columns:   r[4 i], r[4 i + 1] = (row g, columns 8 i + 2 t, + 1), r[4 i + 2], r[4 i + 3] = (row g + 8, the same)
-//   store of 32 columns:  r[2 i] -> (row g, column 4 i + t), r[2 i + 1] -> (row g + 8, column 4 i + t)
-// so 64 fp32 columns that were loaded, rounded to bf16 pairs, are stored as an A operand of 64 rows and K = 64.
+__device__ __forceinline__ void st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+                 "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+// Fragment-shaped accesses of 16 lanes, for accumulators of 64 rows (rows 16 w .. 16 w + 15 live in lanes 32 w .. 32 w + 15) and for
+// operands that arrive in fragments.  Thread 4 g + t of the warp:
+//   load of 8 n columns:  r[4 i], r[4 i + 1] = (lane g, columns 8 i + 2 t, + 1), r[4 i + 2], r[4 i + 3] = (lane g + 8, the same)
+//   store of 8 columns:   r[0], r[1] -> (lanes g and g + 8, column t), r[2], r[3] -> (lanes g and g + 8, column 4 + t)
+// The store's registers are those of an mma.sync A fragment, or of transposed 8 x 8 blocks as ldmatrix loads them: pairs of bf16
+// along K, as an A operand in tensor memory has them.
+__device__ __forceinline__ void ld_frag16(uint32_t taddr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void ld_frag32(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ void ld_frag64(uint32_t taddr, uint32_t* r) {
     asm volatile(
         "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
@@ -117,12 +165,18 @@ __device__ __forceinline__ void ld_frag64(uint32_t taddr, uint32_t* r) {
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void st_frag32(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
+__device__ __forceinline__ void st_frag8(uint32_t taddr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
+}
+
+// Pairs of fp32 in one instruction.
+__device__ __forceinline__ void mul2(uint32_t& x, uint32_t& y, float bx, float by) {
+    asm("{\n.reg .b64 a, b;\nmov.b64 a, {%0,%1};\nmov.b64 b, {%2,%3};\nmul.rn.ftz.f32x2 a, a, b;\nmov.b64 {%0,%1}, a;\n}\n" : "+r"(x), "+r"(y) : "f"(bx), "f"(by));
+}
+__device__ __forceinline__ void sub2(uint32_t& x, uint32_t& y, uint32_t bx, uint32_t by) {   // x - b: the signs of b flipped by a product with -1
+    asm("{\n.reg .b64 a, b, m;\nmov.b64 a, {%0,%1};\nmov.b64 b, {%2,%3};\nmov.b64 m, {%4,%4};\nfma.rn.ftz.f32x2 a, b, m, a;\nmov.b64 {%0,%1}, a;\n}\n"
+        : "+r"(x), "+r"(y)
+        : "r"(bx), "r"(by), "f"(-1.0f));
 }
 
 // ------------------------------------------------------------ tcgen05.mma ----

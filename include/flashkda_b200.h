@@ -204,8 +204,8 @@ int fkda_cp_fold(const float* S, const float* M, const float* N, float* out, int
 
 /* ---- Operators beside the KDA forward (no counterpart in the reference) ----
  *
- * Strides are in elements.  Where a tensor is read in tiles (q, k, v, k_rope, cache) its base address and the strides of its
- * dimensions longer than one are multiples of 16 bytes, and so are those of out; the innermost dimension is contiguous. */
+ * Strides are in elements.  The base addresses of q, k, v, k_rope, cache and out and the strides of their dimensions longer than
+ * one are positive multiples of 16 bytes; the innermost dimension is contiguous. */
 
 /*
  * Linear attention with a decay for each head: S_t = exp(g_t) S_{t-1} + v_t k_t^T, o_t = scale S_t q_t.
