@@ -24,7 +24,10 @@ constexpr int kRows = 2 * kTile;             // query rows of a CTA
 constexpr int kSlotBytes = kTile * 128;      // 128 tokens x 64 dimensions
 constexpr int kSlots = 8;
 constexpr int kKeyTiles = 3, kValueTiles = 2;
-constexpr int kThreads = 320;                // two softmax warpgroups, a loading and a multiplying warp
+constexpr int kThreads = 384;                // two softmax warpgroups, and one with a loading and a multiplying warp
+// Registers of a thread: 168 at launch, then 208 for a row's 128 scores and what is made of them; 2 x 208 + 88 = 3 x 168
+constexpr int kRegsRow = 208, kRegsRest = 88;
+static_assert(2 * kRegsRow + kRegsRest <= 3 * 168, "a block has no more");
 constexpr int kSmem = 1024 + (2 * kKeyTiles + kSlots) * kSlotBytes + 256;
 constexpr uint32_t kS = 0, kO = 256;         // tensor-memory columns: scores (and weights) of the two tiles, outputs
 
@@ -42,7 +45,7 @@ struct PromptArgs {
 };
 
 struct Bars {
-    uint64_t q_full, full[kSlots], empty[kSlots], s_full[2], p_full[2], o_done[2], drained;
+    uint64_t q_full, full[kSlots], empty[kSlots], s_full[2], p_full[2][2], o_done[2], drained;
     uint32_t tmem;
     int abort;
 };
@@ -113,7 +116,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
     if (threadIdx.x == 0) {
         mbar_init(&bar.q_full, 1);
         for (int i = 0; i < kSlots; ++i) mbar_init(&bar.full[i], 1), mbar_init(&bar.empty[i], 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&bar.s_full[i], 1), mbar_init(&bar.p_full[i], kTile), mbar_init(&bar.o_done[i], 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&bar.s_full[i], 1), mbar_init(&bar.p_full[i][0], kTile), mbar_init(&bar.p_full[i][1], kTile), mbar_init(&bar.o_done[i], 1);
         mbar_init(&bar.drained, 1);
         bar.abort = 0;
         mbar_fence_init();
@@ -130,15 +133,17 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
     // key blocks of the two tiles: a row sees the keys up to its own place counted from the ends
     int n[2] = {0, 0};
     if (p.any) {
+#pragma unroll
         for (int w = 0; w < 2; ++w) {
             const int last = min(p.row0 + (w + 1) * kTile, p.len_q);   // one past the tile's last row
-            if (p.row0 + w * kTile >= p.len_q) continue;
             const int seen = a.causal ? min(p.len_k, max(0, p.len_k - p.len_q + last)) : p.len_k;
-            n[w] = (seen + kTile - 1) / kTile;
+            n[w] = p.row0 + w * kTile < p.len_q ? (seen + kTile - 1) / kTile : 0;
         }
     }
     const int blocks = max(n[0], n[1]);
 
+    if (warp >= 8) {
+    regs_dec<kRegsRest>();
     if (warp == 8) {
         // ---- loads: the queries, then for every block its keys (two tiles of the head's, one of the token's) and values ----
         if (blocks > 0 && elect_one()) {
@@ -167,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
     } else if (warp == 9) {
         // ---- products ----
         if (blocks > 0 && elect_one()) {
-            constexpr uint32_t kIdS = idesc(kTile, kTile, false, false), kIdO = idesc(kTile, kTile, false, true);
+            constexpr uint32_t kIdS = idesc(kTile, kTile, false, false), kIdO = idesc(kTile, 64, false, true);
             const uint32_t q_addr = smem_u32(q_smem), ring_addr = smem_u32(ring);
             constexpr int kEach = kKeyTiles + kValueTiles;
             bool ok = wait(&bar.q_full, 0, &bar.abort);
@@ -185,28 +190,31 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
             auto free_slots = [&](int first, int count) {
                 for (int s = first; s < first + count; ++s) commit(&bar.empty[s % kSlots]);
             };
+#pragma unroll
             for (int w = 0; w < 2; ++w)
                 if (n[w] > 0 && ok) scores(w, 0, w == 0 || n[0] == 0);
             free_slots(0, kKeyTiles);
             for (int i = 0; i < blocks && ok; ++i) {
                 const int first_v = i < n[0] ? 0 : 1, last_v = i < n[1] ? 1 : 0;
                 const int first_k = i + 1 < n[0] ? 0 : 1, last_k = i + 1 < n[1] ? 1 : 0;
-                for (int w = 0; w < 2 && ok; ++w) {
-                    if (i >= n[w]) continue;
-                    ok = wait(&bar.p_full[w], i & 1, &bar.abort);
-                    if (!ok) break;
-                    for (int c = 0; c < kValueTiles && w == first_v && ok; ++c) {
-                        const int s = i * kEach + kKeyTiles + c;
-                        ok = wait(&bar.full[s % kSlots], (s / kSlots) & 1, &bar.abort);
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    if (i >= n[w] || !ok) continue;
+                    for (int half = 0; half < 2 && ok; ++half) {   // 64 keys
+                        ok = wait(&bar.p_full[w][half], i & 1, &bar.abort);
+                        for (int c = 0; c < kValueTiles && half == 0 && w == first_v && ok; ++c) {
+                            const int s = i * kEach + kKeyTiles + c;
+                            ok = wait(&bar.full[s % kSlots], (s / kSlots) & 1, &bar.abort);
+                        }
+                        if (!ok) break;
+                        fence_after();
+                        for (int c = 0; c < kValueTiles; ++c) {   // 64 dimensions at a time: the two tiles need not be neighbours in the ring
+                            const uint32_t v_addr = ring_addr + ((i * kEach + kKeyTiles + c) % kSlots) * kSlotBytes;
+                            for (int k = 4 * half; k < 4 * half + 4; ++k)
+                                mma_ts(tmem + kO + w * kTile + c * 64, tmem + kS + w * kTile + k * 8, desc(v_addr + k * 2048), kIdO, i > 0 || k > 0);
+                        }
                     }
                     if (!ok) break;
-                    fence_after();
-                    for (int c = 0; c < kValueTiles; ++c) {   // N = 64 dimensions at a time: the two tiles need not be neighbours in the ring
-                        const uint32_t v_addr = ring_addr + ((i * kEach + kKeyTiles + c) % kSlots) * kSlotBytes;
-                        for (int k = 0; k < 8; ++k)
-                            mma_ts(tmem + kO + w * kTile + c * 64, tmem + kS + w * kTile + k * 8, desc(v_addr + k * 2048),
-                                   idesc(kTile, 64, false, true), i > 0 || k > 0);
-                    }
                     commit(&bar.o_done[w]);
                     if (w == last_v) free_slots(i * kEach + kKeyTiles, kValueTiles);
                     if (i + 1 < n[w]) {
@@ -215,13 +223,14 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
                     }
                 }
             }
-            (void)kIdO;
             commit(&bar.drained);
             drain(&bar.drained, 0);
         }
+    }
     } else {
         // ---- weights: thread = row ----
-        const int w = warp >> 2;
+        regs_inc<kRegsRow>();
+        const int w = warp >> 2, n0 = n[0], blocks_w = w == 0 ? n[0] : n[1];
         const int row = p.row0 + w * kTile + (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + kS + w * kTile + lanes, to = tmem + kO + w * kTile + lanes;
@@ -231,8 +240,9 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
         const int least = p.any ? (a.causal ? p.len_k - p.len_q + p.row0 + w * kTile + 1 : p.len_k) : 0;   // what the tile's first row sees
         const float step = 8.0f / c;
         float top = -INFINITY, sum = 0.0f;
-        uint32_t s[128];
-        for (int i = 0; i < n[w]; ++i) {
+#pragma unroll 1
+        for (int i = 0; i < blocks_w; ++i) {
+            uint32_t s[128];
             if (i > 0) wait_warp(&bar.o_done[w], (i - 1) & 1, &bar.abort);   // (issued in front of these scores)
             wait_warp(&bar.s_full[w], i & 1, &bar.abort);
             fence_after();
@@ -243,9 +253,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
 #pragma unroll
                 for (int k = 0; k < 128; ++k) s[k] = i * kTile + k < seen ? s[k] : 0xff800000u;
             }
-            float m = f(s[0]);
+            float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int k = 1; k < 128; ++k) m = fmaxf(m, f(s[k]));
+            for (int k = 0; k < 128; k += 2) most[(k >> 1) & 3] = fmaxf(fmaxf(f(s[k]), f(s[k + 1])), most[(k >> 1) & 3]);
+            const float m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
             // the reference moves where the maximum is 2^8 above it; then what was summed so far is scaled down
             const bool move = m > top + step || (top == -INFINITY && m > -INFINITY);
             if (__any_sync(0xffffffffu, move)) {
@@ -265,20 +276,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
                 }
             }
             const float ref = top == -INFINITY ? 0.0f : -top * c;
-            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int k = 0; k < 128; ++k) {
-                const float e = ex2_approx(__fmaf_rn(f(s[k]), c, ref));
-                part[k & 3] += e;
-                s[k] = u(e);
-            }
-            sum += (part[0] + part[1]) + (part[2] + part[3]);
-#pragma unroll
-            for (int k = 0; k < 64; ++k) s[k] = pack_bf2(f(s[2 * k]), f(s[2 * k + 1]));
-            st32(ts, s);
-            st32(ts + 32, s + 32);
             // values behind the sequence's last key are another sequence's, or nobody's: nothing times them must be nothing
-            if ((i + 1) * kTile > p.len_k && w == (i < n[0] ? 0 : 1)) {
+            if ((i + 1) * kTile > p.len_k && w == (i < n0 ? 0 : 1)) {
                 const int from = p.len_k - i * kTile;
                 for (int v = 0; v < kValueTiles; ++v) {
                     const int sl = i * (kKeyTiles + kValueTiles) + kKeyTiles + v;
@@ -288,12 +287,27 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
                 }
                 fence_proxy_async_smem();
             }
-            wait_st();
-            fence_before();
-            arrive(&bar.p_full[w]);
+            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {   // the product with the values starts on the first 64 keys
+                uint32_t* x = s + half * 64;
+#pragma unroll
+                for (int k = 0; k < 64; k += 2) {
+                    fma2(x[k], x[k + 1], c, ref);
+                    x[k] = u(ex2_approx(f(x[k])));
+                    x[k + 1] = u(ex2_approx(f(x[k + 1])));
+                    add2(part[k & 2], part[(k & 2) + 1], x[k], x[k + 1]);
+                    x[k >> 1] = pack_bf2(f(x[k]), f(x[k + 1]));
+                }
+                st32(ts + half * 32, x);
+                wait_st();
+                fence_before();
+                arrive(&bar.p_full[w][half]);
+            }
+            sum += (part[0] + part[1]) + (part[2] + part[3]);
         }
-        if (n[w] > 0) {
-            wait_warp(&bar.o_done[w], (n[w] - 1) & 1, &bar.abort);
+        if (blocks_w > 0) {
+            wait_warp(&bar.o_done[w], (blocks_w - 1) & 1, &bar.abort);
             fence_after();
         }
         const bool mine = p.any && row < p.len_q;
@@ -303,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             uint32_t o[32];
-            if (n[w] > 0) {
+            if (blocks_w > 0) {
                 ld32(to + k * 32, o);
                 wait_ld();
             } else {

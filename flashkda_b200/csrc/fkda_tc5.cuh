@@ -169,7 +169,22 @@ __device__ __forceinline__ void st_frag8(uint32_t taddr, uint32_t r0, uint32_t r
     asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
 }
 
+// A warpgroup's registers per thread from here on: `inc` waits until others have given up as many (the shares of all warpgroups of a
+// block may not add up to more than it was launched with).
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 // Pairs of fp32 in one instruction.
+__device__ __forceinline__ void fma2(uint32_t& x, uint32_t& y, float b, float c) {   // x b + c, y b + c
+    asm("{\n.reg .b64 a, b, c;\nmov.b64 a, {%0,%1};\nmov.b64 b, {%2,%2};\nmov.b64 c, {%3,%3};\nfma.rn.ftz.f32x2 a, a, b, c;\nmov.b64 {%0,%1}, a;\n}\n"
+        : "+r"(x), "+r"(y)
+        : "f"(b), "f"(c));
+}
+__device__ __forceinline__ void add2(float& x, float& y, uint32_t bx, uint32_t by) {
+    asm("{\n.reg .b64 a, b;\nmov.b64 a, {%0,%1};\nmov.b64 b, {%2,%3};\nadd.rn.ftz.f32x2 a, a, b;\nmov.b64 {%0,%1}, a;\n}\n" : "+f"(x), "+f"(y) : "r"(bx), "r"(by));
+}
 __device__ __forceinline__ void mul2(uint32_t& x, uint32_t& y, float bx, float by) {
     asm("{\n.reg .b64 a, b;\nmov.b64 a, {%0,%1};\nmov.b64 b, {%2,%3};\nmul.rn.ftz.f32x2 a, a, b;\nmov.b64 {%0,%1}, a;\n}\n" : "+r"(x), "+r"(y) : "f"(bx), "f"(by));
 }
