@@ -15,6 +15,8 @@
 //
 // Numerics: as in the expanded form (fp32 scores, sums and outputs; weights against a reference within 2^8 of the running maximum,
 // rounded to bf16 for the value product only); parts are joined in fp32 in the order of the tokens.
+#include <algorithm>
+
 #include "fkda_tc5.cuh"
 
 namespace fkda {
@@ -27,7 +29,8 @@ constexpr int kWidth = 576, kValue = 512;
 constexpr int kChunks = kWidth / 64;         // 64-dimension tiles of a row or token
 constexpr int kChunkBytes = 64 * 128;
 constexpr int kStageBytes = kChunks * kChunkBytes;
-constexpr int kStages = 2;
+constexpr int kStages = 2;                   // (tile g's is g & 1)
+constexpr int kGroups = 5;                   // of a stage, loaded and freed apart: four pairs of 64-dimension tiles, and the rotated one
 constexpr int kThreads = 192;                // softmax warpgroup, a loading and a multiplying warp
 constexpr int kMaxSeqs = kStages * kStageBytes / 4;   // tile counts of all sequences pass through the stages' memory
 constexpr uint32_t kO = 0, kS = 256;         // tensor-memory columns: four output accumulators, two score buffers
@@ -36,7 +39,10 @@ struct DecodeArgs {
     __nv_bfloat16* out;
     float* lse;
     const int32_t *table, *lens;
+    const __nv_bfloat16* cache;
+    int64_t page_stride;     // elements from page to page where a page's tokens lie one behind the other, else 0 (no fetching ahead)
     float* parts;        // [CTAs][2][kRows][kValue], then their lse [CTAs][2][kRows]
+    int64_t* prefix;     // [B + 1] tiles in front of each sequence, and of all
     int64_t out_batch, out_row, table_stride, pages;
     int B, Tq, H, R, row_tiles, groups, page, box, max_pages;
     float scale;
@@ -45,14 +51,14 @@ struct DecodeMaps {
     CUtensorMap q, cache;
 };
 struct Bars {
-    uint64_t q_full, q_empty, full[kStages], empty[kStages], s_full[2], p_full, o_done, drained;
+    uint64_t q_full, q_empty, full[kStages][kGroups], empty[kStages][kGroups], s_full[2], p_full, o_done, drained;
     uint32_t tmem;
     int abort;
     int first_seq, first_tile, count;
-    float factor[kRows];
+    alignas(16) float factor[kRows];
 };
-constexpr int kSmem = 1024 + kStageBytes + kStages * kStageBytes + kChunkBytes + 512;
-static_assert(sizeof(Bars) <= 512, "barriers");
+constexpr int kSmem = kStageBytes + kStages * kStageBytes + kChunkBytes + 640;
+static_assert(sizeof(Bars) <= 640 && kSmem <= 232448, "shared memory of an SM");
 
 __device__ __forceinline__ int tiles_of(int len) { return len > 0 ? (len + kTok - 1) / kTok : 0; }
 // Length of a sequence as far as its pages go.
@@ -86,17 +92,17 @@ struct Walk {
 };
 
 __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ DecodeMaps maps) {
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* q_smem = smem;                       // [9][64 rows][128 bytes]
     uint8_t* stages = smem + kStageBytes;         // [2][9][64 tokens][128 bytes]
     uint8_t* p_smem = stages + kStages * kStageBytes;
     Bars& bar = *reinterpret_cast<Bars*>(p_smem + kChunkBytes);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         mbar_init(&bar.q_full, 1);
         mbar_init(&bar.q_empty, 1);
-        for (int i = 0; i < kStages; ++i) mbar_init(&bar.full[i], 1), mbar_init(&bar.empty[i], 1);
+        for (int i = 0; i < kStages; ++i)
+            for (int j = 0; j < kGroups; ++j) mbar_init(&bar.full[i][j], 1), mbar_init(&bar.empty[i][j], 1);
         for (int i = 0; i < 2; ++i) mbar_init(&bar.s_full[i], 1);
         mbar_init(&bar.p_full, 128);
         mbar_init(&bar.o_done, 1);
@@ -122,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
         const int64_t share = (total + a.groups - 1) / a.groups, mine = share * group;
         int64_t seen = 0;
-        for (int base = 0; base < a.B && mine < total; base += 32) {
+        for (int base = 0; base < a.B; base += 32) {
             const int c = base + lane < a.B ? counts[base + lane] : 0;
             int upto = c;
 #pragma unroll
@@ -130,106 +136,155 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
                 const int x = __shfl_up_sync(0xffffffffu, upto, off);
                 if (lane >= off) upto += x;
             }
-            const uint32_t behind = __ballot_sync(0xffffffffu, seen + upto > mine);
-            if (behind != 0) {
-                if (lane == __ffs(behind) - 1) {
-                    bar.first_seq = base + lane;
-                    bar.first_tile = (int)(mine - (seen + upto - c));
-                    bar.count = (int)min(share, total - mine);
-                }
-                break;
+            const int64_t before = seen + upto - c;
+            if (mine < total && before <= mine && mine < before + c) {
+                bar.first_seq = base + lane;
+                bar.first_tile = (int)(mine - before);
+                bar.count = (int)min(share, total - mine);
             }
+            if (blockIdx.x == 0 && base + lane < a.B) a.prefix[base + lane] = before;
             seen += __shfl_sync(0xffffffffu, upto, 31);
         }
+        if (blockIdx.x == 0 && lane == 0) a.prefix[a.B] = total;
     }
     fence_proxy_async_smem();   // (the stages are written by copies from here on)
     __syncthreads();
-    const uint32_t tmem = bar.tmem;
-    Walk walk{bar.first_seq, bar.first_tile, bar.count, 0, 0, 0};
+    constexpr uint32_t tmem = 0;   // (all columns are this CTA's)
+    Walk walk{(int)uniform(bar.first_seq), (int)uniform(bar.first_tile), as_assumed(smem, bar.tmem) ? (int)uniform(bar.count) : 0, 0, 0, 0};
 
     if (warp == 4) {
-        // ---- loads ----
-        int g = 0, pieces = 0;
+        // ---- loads: a tile in groups of its dimensions, box by box (pages may end inside it); two tiles on are fetched into L2, so that a
+        //      stage that was freed is full again without waiting for HBM ----
+        const uint32_t q_addr = smem_u32(q_smem), st_addr = smem_u32(stages), leader = elect_one();
+        const int boxes = kTok / a.box;
+        int g = 0, pieces = 0, asked = 0, issued = 0;
         bool ok = true;
+        auto page_of = [&](int tok) {
+            const int page = a.table[(int64_t)walk.b * a.table_stride + tok / a.page];
+            return page < 0 || page >= a.pages ? 0 : page;
+        };
+        auto fetch_ahead = [&](int t) {   // lane = box of the tile
+            const int tok = t * kTok + lane * a.box;
+            if (a.page_stride == 0 || t >= walk.until || lane >= boxes || tok >= walk.len) return;
+            const __nv_bfloat16* from = a.cache + (int64_t)page_of(tok) * a.page_stride + (int64_t)(tok % a.page) * kWidth;
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"(a.box * kWidth * 2) : "memory");
+        };
+#pragma unroll 1
         for (; ok && walk.next(a); walk.done(), ++pieces) {
-            if (pieces > 0) ok = wait(&bar.q_empty, (pieces - 1) & 1, &bar.abort);
-            ok = __all_sync(0xffffffffu, ok);
+            fetch_ahead(walk.t + 1);
+            __syncwarp();
+            if (pieces > 0) ok = __all_sync(0xffffffffu, wait(&bar.q_empty, (pieces - 1) & 1, &bar.abort));
             if (!ok) break;
-            if (lane == 0) {
-                mbar_arrive_expect_tx(&bar.q_full, kStageBytes);
-                for (int c = 0; c < kChunks; ++c) tma_load_3d(q_smem + c * kChunkBytes, &maps.q, c * 64, rt * kRows, walk.b, &bar.q_full);
-            }
-            const int boxes = kTok / a.box;
+            expect(&bar.q_full, kStageBytes, leader);
+            ++asked;
+            const int seq = uniform(walk.b);
+#pragma unroll 1
+            for (int c = 0; c < kChunks; ++c) load_3d(q_addr + c * kChunkBytes, &maps.q, c * 64, rt * kRows, seq, &bar.q_full, leader);
+#pragma unroll 1
             for (int t = walk.t; t < walk.until; ++t, ++g) {
-                const int stage = g % kStages;
-                const int tok = t * kTok + lane * a.box;   // lane = box of the tile
+                const int tok = t * kTok + lane * a.box;
                 const bool load = lane < boxes && tok < walk.len;
-                int page = 0;
-                if (load) {
-                    page = a.table[(int64_t)walk.b * a.table_stride + tok / a.page];
-                    page = page < 0 || page >= a.pages ? 0 : page;
+                const int my_page = load ? page_of(tok) : 0, my_row = load ? tok % a.page : 0, n = __popc(__ballot_sync(0xffffffffu, load));
+                fetch_ahead(t + 2);
+                __syncwarp();
+#pragma unroll 1
+                for (int j = 0; j < kGroups; ++j) {
+                    if (g >= kStages) ok = __all_sync(0xffffffffu, wait(&bar.empty[g & 1][j], ((g >> 1) - 1) & 1, &bar.abort));
+                    if (!ok) break;
+                    const int width = j == kGroups - 1 ? 1 : 2;
+                    uint64_t* full = &bar.full[g & 1][j];
+                    expect(full, n * a.box * 128 * width, leader);
+#pragma unroll 1
+                    for (int b = 0; b < n; ++b) {
+                        const int page = __shfl_sync(0xffffffffu, my_page, b), row = __shfl_sync(0xffffffffu, my_row, b);
+                        const uint32_t dst = st_addr + (g & 1) * kStageBytes + 2 * j * kChunkBytes + b * a.box * 128;
+                        load_3d(dst, &maps.cache, j * 128, row, page, full, leader);
+                        if (width == 2) load_3d(dst + kChunkBytes, &maps.cache, j * 128 + 64, row, page, full, leader);
+                    }
+                    issued = g * kGroups + j + 1;
                 }
-                if (g >= kStages) ok = wait(&bar.empty[stage], (g / kStages - 1) & 1, &bar.abort);
-                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                const int n = __popc(__ballot_sync(0xffffffffu, load));
-                if (lane == 0) mbar_arrive_expect_tx(&bar.full[stage], n * a.box * kWidth * 2);
-                __syncwarp();
-                if (load) {
-                    uint8_t* dst = stages + stage * kStageBytes + lane * a.box * 128;
-                    for (int c = 0; c < kChunks; ++c) tma_load_3d(dst + c * kChunkBytes, &maps.cache, c * 64, tok % a.page, page, &bar.full[stage]);
-                }
-                __syncwarp();
             }
             if (!ok) break;
         }
-        if (lane == 0) {
-            if (pieces > 0) drain(&bar.q_full, (pieces - 1) & 1);
-            for (int k = max(0, g - kStages); k < g; ++k) drain(&bar.full[k % kStages], (k / kStages) & 1);
-        }
+        if (asked > 0) drain(&bar.q_full, (asked - 1) & 1);
+#pragma unroll 1
+        for (int k = max(0, issued - kStages * kGroups); k < issued; ++k) drain(&bar.full[k / kGroups % kStages][k % kGroups], (k / kGroups / kStages) & 1);
         __syncwarp();
     } else if (warp == 5) {
-        // ---- products ----
-        if (elect_one()) {
-            constexpr uint32_t kIdS = idesc(kRows, kTok, false, false), kIdO = idesc(128, kRows, true, false);
-            const uint32_t q_addr = smem_u32(q_smem), st_addr = smem_u32(stages), p_addr = smem_u32(p_smem);
-            int g = 0;          // tiles whose scores have been issued
-            int done = 0;       // tiles whose value product has been issued
-            int piece = 0;
-            bool ok = true, prev_first = false;
-            auto values = [&](bool first) {   // the value product of tile `done`
-                ok = wait(&bar.p_full, done & 1, &bar.abort);
-                if (!ok) return;
+        // ---- products: two lines of work, each taken up as soon as what it waits for is there: the scores of tile `g`, group by group of its
+        //      dimensions, at most one tile ahead of the value product of tile `done` ----
+        constexpr uint32_t kIdS = idesc(kRows, kTok, false, false), kIdO = idesc(128, kRows, true, false);
+        const uint32_t q_desc = desc(smem_u32(q_smem)), k_desc = desc(smem_u32(stages)), leader = elect_one();
+        const uint32_t v_desc = desc(smem_u32(stages), kChunkBytes), p_desc = desc(smem_u32(p_smem));
+        int g = 0, group_of = 0, done = 0, piece = 0;
+        bool more = walk.next(a), fresh = true;           // `fresh`: the next scores are a stretch's first
+        int start = walk.t;
+        uint32_t firsts = 0;                               // bit per score buffer: whether its tile's value product starts an output
+        uint32_t idle = 0;
+        long long since = 0;
+        while (more || done < g) {
+            // what is there: the groups of tile `g` (bits 0 to 4), the weights of tile `done` (5), the stretch's queries (6)
+            uint64_t* look = lane < kGroups ? &bar.full[g & 1][lane] : (lane == 5 ? &bar.p_full : &bar.q_full);
+            const int phase = lane < kGroups ? g >> 1 : (lane == 5 ? done : piece);
+            const uint32_t there = __ballot_sync(0xffffffffu, mbar_test_wait(look, phase & 1));
+            const int scored = g;   // (`there` speaks of the weights of a tile whose scores had been issued)
+            bool moved = false;
+            if (more && g <= done + 1 && (!fresh || group_of > 0 || (there >> 6 & 1) != 0) && (there >> group_of & 1) != 0) {
                 fence_after();
-                const uint32_t stage = st_addr + (done % kStages) * kStageBytes;
-                for (int m = 0; m < 4; ++m)
-                    for (int k = 0; k < 4; ++k)
-                        mma_ss(tmem + kO + m * kRows, desc(stage + 2 * m * kChunkBytes + k * 2048, kChunkBytes), desc(p_addr + k * 32), kIdO, !first || k > 0);
-                commit(&bar.empty[done % kStages]);
-                commit(&bar.o_done);
-                ++done;
-            };
-            for (; ok && walk.next(a); walk.done(), ++piece) {
-                ok = wait(&bar.q_full, piece & 1, &bar.abort);
-                for (int t = walk.t; t < walk.until && ok; ++t) {
-                    ok = wait(&bar.full[g % kStages], (g / kStages) & 1, &bar.abort);
-                    if (!ok) break;
-                    fence_after();
-                    const uint32_t stage = st_addr + (g % kStages) * kStageBytes;
-                    for (int c = 0; c < kChunks; ++c)
-                        for (int k = 0; k < 4; ++k)
-                            mma_ss(tmem + kS + (g & 1) * kTok, desc(q_addr + c * kChunkBytes + k * 32), desc(stage + c * kChunkBytes + k * 32), kIdS, (c | k) != 0);
-                    commit(&bar.s_full[g & 1]);
-                    if (t + 1 == walk.until) commit(&bar.q_empty);
-                    if (g > 0) values(prev_first);
-                    prev_first = t == walk.t;
+                const uint32_t to = tmem + kS + (g & 1) * kTok, q = q_desc + group_of * (2 * kChunkBytes / 16),
+                               k_ = k_desc + (g & 1) * (kStageBytes / 16) + group_of * (2 * kChunkBytes / 16);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mma_ss(to, q + k * 32 / 16, k_ + k * 32 / 16, kIdS, (group_of | k) != 0, leader);
+                if (group_of < kGroups - 1) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mma_ss(to, q + (kChunkBytes + k * 32) / 16, k_ + (kChunkBytes + k * 32) / 16, kIdS, 1, leader);
+                    ++group_of;
+                } else {
+                    commit(&bar.s_full[g & 1], leader);
+                    commit(&bar.empty[g & 1][kGroups - 1], leader);
+                    firsts = (firsts & ~(1u << (g & 1))) | (uint32_t)fresh << (g & 1);
+                    group_of = 0;
+                    fresh = false;
                     ++g;
+                    if (++walk.t == walk.until) {
+                        commit(&bar.q_empty, leader);
+                        walk.left -= walk.until - start;
+                        more = walk.next(a);
+                        start = walk.t;
+                        fresh = true;
+                        ++piece;
+                    }
                 }
+                moved = true;
             }
-            if (ok && g > 0) values(prev_first);
-            commit(&bar.drained);
-            drain(&bar.drained, 0);
+            if (done < scored && (there >> 5 & 1) != 0) {
+                fence_after();
+                const uint32_t v = v_desc + (done & 1) * (kStageBytes / 16), adds = (firsts >> (done & 1) & 1) ^ 1;
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mma_ss(tmem + kO + m * kRows, v + (2 * m * kChunkBytes + k * 2048) / 16, p_desc + k * 32 / 16, kIdO, k > 0 ? 1 : adds, leader);
+                    commit(&bar.empty[done & 1][m], leader);
+                }
+                commit(&bar.o_done, leader);
+                ++done;
+                moved = true;
+            }
+            if (moved) {
+                idle = 0;
+            } else if ((++idle & 255u) == 0) {
+                const long long now = clock64();
+                if (idle == 256u) since = now;
+                bool ok = *reinterpret_cast<volatile int*>(&bar.abort) == 0;
+                if (now - since > kWaitCycles) ok = give_up(&bar.abort);
+                if (!__all_sync(0xffffffffu, ok)) break;
+            }
         }
+        commit(&bar.drained, leader);
+        drain(&bar.drained, 0);
+        __syncwarp();
     } else {
         // ---- weights: warp w has rows 16 w .. 16 w + 15 of the tile, thread 4 g + t columns 8 i + 2 t, + 1 of rows g and g + 8 ----
         const int gr = lane >> 2, tc = lane & 3;
@@ -331,21 +386,56 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
             named_sync(1, 128);
             wait_warp(&bar.o_done, (g - 1) & 1, &bar.abort);
             fence_after();
+            if (whole) {
+                // 16 dimensions x 32 rows at a time as fragments, stored transposed: a row's 32 dimensions of the warp leave as 64 bytes
+                uint8_t* stage = p_smem + warp * 2048;   // [32 rows][64 bytes], the weights' place
+                const int token = (lane & 7) + ((lane >> 4) << 3);
+                __nv_bfloat16* dst = a.out + (int64_t)walk.b * a.out_batch + (int64_t)(rt * kRows) * a.out_row + warp * 32;
 #pragma unroll 1
-            for (int k = 0; k < 8; ++k) {
-                uint32_t o[32];
-                ld32(tmem + kO + k * 32 + lanes, o);
-                wait_ld();
-                const int dim = (k >> 1) * 128 + warp * 32 + lane, r0 = (k & 1) * 32;
-                if (whole) {
-                    __nv_bfloat16* dst = a.out + (int64_t)walk.b * a.out_batch + (int64_t)(rt * kRows + r0) * a.out_row + dim;
+                for (int k = 0; k < 8; ++k) {
+                    const int r0 = (k & 1) * 32;
+#pragma unroll
+                    for (int up = 0; up < 2; ++up) {
+                        uint32_t o[16];
+                        ld_frag32(tmem + kO + k * 32 + lanes + ((uint32_t)(up * 16) << 16), o);
+                        wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {   // 16 rows
+                            uint32_t y[4];
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                const float2 e = *reinterpret_cast<const float2*>(&bar.factor[r0 + i * 16 + j * 8 + 2 * tc]);
+                                const uint32_t* x = o + 8 * i + 4 * j;
+                                y[2 * j] = pack_bf2(f(x[0]) * e.x, f(x[1]) * e.y);
+                                y[2 * j + 1] = pack_bf2(f(x[2]) * e.x, f(x[3]) * e.y);
+                            }
+                            const int to = i * 16 + token, unit = up * 2 + ((lane >> 3) & 1);
+                            asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(smem_u32(stage + to * 64 + ((unit ^ ((to >> 1) & 3)) << 4))), "r"(y[0]),
+                                         "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
+                        }
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int row_of = i * 8 + (lane >> 2), unit = lane & 3;
+                        const uint4 x = *reinterpret_cast<const uint4*>(stage + row_of * 64 + ((unit ^ ((row_of >> 1) & 3)) << 4));
+                        if (rt * kRows + r0 + row_of < a.R) *reinterpret_cast<uint4*>(dst + (int64_t)(r0 + row_of) * a.out_row + (k >> 1) * 128 + unit * 8) = x;
+                    }
+                    __syncwarp();
+                }
+            } else {
+                const int rows = min(kRows, a.R - rt * kRows);
+#pragma unroll 1
+                for (int k = 0; k < 8; ++k) {
+                    const int r0 = (k & 1) * 32;
+                    if (r0 >= rows) continue;
+                    uint32_t o[32];
+                    ld32(tmem + kO + k * 32 + lanes, o);
+                    wait_ld();
+                    float* to = part + r0 * kValue + (k >> 1) * 128 + warp * 32 + lane;
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
-                        if (rt * kRows + r0 + j < a.R) dst[j * a.out_row] = f2bf(f(o[j]) * bar.factor[r0 + j]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (rt * kRows + r0 + j < a.R) part[(r0 + j) * kValue + dim] = f(o[j]) * bar.factor[r0 + j];
+                        if (r0 + j < rows) to[j * kValue] = f(o[j]) * bar.factor[r0 + j];
                 }
             }
             fence_before();
@@ -357,74 +447,65 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     if (warp == 5) tmem_dealloc(tmem, 512);
 }
 
-// Joins the parts of the sequences that a cut runs through, and writes those without any token.  A CTA: eight rows of a sequence, a
-// warp each.
-__global__ void __launch_bounds__(256) latent_join_kernel(const __grid_constant__ DecodeArgs a, int ctas) {
-    __shared__ int64_t sums[2][8];
+// Joins the parts of the sequences that a cut runs through, and writes those without any token.  A CTA has some rows of a sequence and
+// eight groups of 128 threads, with four dimensions each: as many groups share a row, taking its parts in turn, as there are parts.
+constexpr int kJoinGroups = 8;
+__global__ void __launch_bounds__(128 * kJoinGroups) latent_join_kernel(const __grid_constant__ DecodeArgs a, int ctas, int rows_each) {
+    __shared__ float4 sums[kJoinGroups][128];
     grid_dep_launch();
     grid_dep_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int per = (a.R + 7) / 8, b = (int)(blockIdx.x / per), r = (int)(blockIdx.x % per) * 8 + warp;
-    int64_t total = 0, before = 0;
-    for (int k = threadIdx.x; k < a.B; k += 256) {
-        const int n = tiles_of(length(a, k));
-        total += n;
-        if (k < b) before += n;
-    }
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) {
-        total += __shfl_xor_sync(0xffffffffu, total, off);
-        before += __shfl_xor_sync(0xffffffffu, before, off);
-    }
-    if (lane == 0) sums[0][warp] = total, sums[1][warp] = before;
-    __syncthreads();
-    total = before = 0;
-    for (int k = 0; k < 8; ++k) total += sums[0][k], before += sums[1][k];
-    if (r >= a.R) return;
+    const int per = (a.R + rows_each - 1) / rows_each, b = (int)(blockIdx.x / per), r0 = (int)(blockIdx.x % per) * rows_each;
+    const int me = threadIdx.x & 127, group = threadIdx.x >> 7;
     const int n = tiles_of(length(a, b));
-    __nv_bfloat16* dst = a.out + (int64_t)b * a.out_batch + (int64_t)r * a.out_row;
-    float* lse = a.lse != nullptr ? a.lse + (int64_t)b * a.R + r : nullptr;
-    if (n == 0) {
-        for (int k = lane; k < kValue / 8; k += 32) *reinterpret_cast<uint4*>(dst + k * 8) = make_uint4(0, 0, 0, 0);
-        if (lane == 0 && lse != nullptr) *lse = -INFINITY;
-        return;
-    }
+    const int64_t before = a.prefix[b], total = a.prefix[a.B];
     const int64_t share = (total + a.groups - 1) / a.groups;
-    const int64_t first = before / share, last = (before + n - 1) / share;
-    if (first == last) return;
-    const int rt = r / kRows, row = r % kRows;
+    const int64_t first = n > 0 ? before / share : 0, last = n > 0 ? (before + n - 1) / share : 0;
+    if (n > 0 && first == last) return;
     const float* lses = a.parts + (int64_t)ctas * 2 * kRows * kValue;
-    auto slot = [&](int64_t x) { return (x * a.row_tiles + rt) * 2 + (x * share >= before ? 0 : 1); };   // (a CTA's first stretch is its slot 0)
-    float top = -INFINITY;
-    for (int64_t x = first + lane; x <= last; x += 32) top = fmaxf(top, lses[slot(x) * kRows + row]);
+    const int parts = (int)min(last - first + 1, (int64_t)kJoinGroups);
+    const int sharing = parts > 4 ? 8 : (parts > 2 ? 4 : (parts > 1 ? 2 : 1)), mine = group % sharing;
+    const int end = min(a.R, r0 + rows_each);
+    for (int base = r0; base < end; base += kJoinGroups / sharing) {   // (all threads come as often to the barriers)
+        const int r = base + group / sharing, rt = r / kRows, row = r % kRows;
+        auto slot = [&](int64_t x) { return ((x * a.row_tiles + rt) * 2 + (x * share >= before ? 0 : 1)) * kRows + row; };   // (a CTA's first stretch is its slot 0)
+        float ref = -INFINITY, sum = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (n > 0 && r < end) {
+            for (int64_t x = first + (threadIdx.x & 31); x <= last; x += 32) ref = fmaxf(ref, lses[slot(x)]);
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, acc[16];
+            for (int off = 16; off >= 1; off >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, off));
+            if (ref == -INFINITY) ref = 0.0f;
+            for (int64_t x = first + (threadIdx.x & 31); x <= last; x += 32) sum += expf(lses[slot(x)] - ref);
 #pragma unroll
-    for (int k = 0; k < 16; ++k) acc[k] = 0.0f;
-    for (int64_t x = first; x <= last; ++x) {
-        const int64_t s = slot(x);
-        const float z = lses[s * kRows + row];
-        if (z == -INFINITY) continue;
-        const float w = expf(z - ref);
-        sum += w;
-        const float* src = a.parts + (s * kRows + row) * kValue;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float4 v = *reinterpret_cast<const float4*>(src + k * 128 + lane * 4);
-            acc[4 * k] += w * v.x;
-            acc[4 * k + 1] += w * v.y;
-            acc[4 * k + 2] += w * v.z;
-            acc[4 * k + 3] += w * v.w;
+            for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+#pragma unroll 4
+            for (int64_t x = first + mine; x <= last; x += sharing) {
+                const int64_t s = slot(x);
+                const float w = expf(lses[s] - ref);
+                const float4 v = *reinterpret_cast<const float4*>(a.parts + s * kValue + me * 4);
+                acc.x += w * v.x;
+                acc.y += w * v.y;
+                acc.z += w * v.z;
+                acc.w += w * v.w;
+            }
         }
+        sums[group][me] = acc;
+        __syncthreads();
+        if (mine == 0 && r < end) {
+            for (int k = 1; k < sharing; ++k) {
+                const float4 v = sums[group + k][me];
+                acc.x += v.x;
+                acc.y += v.y;
+                acc.z += v.z;
+                acc.w += v.w;
+            }
+            const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+            *reinterpret_cast<uint2*>(a.out + (int64_t)b * a.out_batch + (int64_t)r * a.out_row + me * 4) =
+                make_uint2(pack_bf2(acc.x * inv, acc.y * inv), pack_bf2(acc.z * inv, acc.w * inv));
+            if (me == 0 && a.lse != nullptr) a.lse[(int64_t)b * a.R + r] = sum == 0.0f ? -INFINITY : ref + logf(sum);
+        }
+        __syncthreads();
     }
-    const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-        *reinterpret_cast<uint2*>(dst + k * 128 + lane * 4) =
-            make_uint2(pack_bf2(acc[4 * k] * inv, acc[4 * k + 1] * inv), pack_bf2(acc[4 * k + 2] * inv, acc[4 * k + 3] * inv));
-    if (lane == 0 && lse != nullptr) *lse = sum == 0.0f ? -INFINITY : ref + logf(sum);
 }
 
 int groups_for(int64_t row_tiles) {
@@ -436,7 +517,7 @@ int groups_for(int64_t row_tiles) {
 
 size_t latent_decode_workspace(const fkda_latent_decode_params& p) {
     const int64_t row_tiles = (p.Tq * p.H + kRows - 1) / kRows;
-    return (size_t)(row_tiles * groups_for(row_tiles)) * 2 * kRows * (kValue + 1) * sizeof(float);
+    return (size_t)(row_tiles * groups_for(row_tiles)) * 2 * kRows * (kValue + 1) * sizeof(float) + (size_t)(p.B + 1) * sizeof(int64_t);
 }
 
 int launch_latent_decode(const fkda_latent_decode_params& p, cudaStream_t stream, int* n_launches) {
@@ -445,6 +526,8 @@ int launch_latent_decode(const fkda_latent_decode_params& p, cudaStream_t stream
     a.out = static_cast<__nv_bfloat16*>(p.out);
     a.lse = p.lse;
     a.table = p.block_table;
+    a.cache = static_cast<const __nv_bfloat16*>(p.cache);
+    a.page_stride = p.cache_stride[1] == kWidth ? p.cache_stride[0] : 0;
     a.lens = p.cache_lens;
     a.parts = static_cast<float*>(p.workspace);
     a.out_batch = p.out_stride[0];
@@ -458,6 +541,7 @@ int launch_latent_decode(const fkda_latent_decode_params& p, cudaStream_t stream
     a.box = p.page_size % 64 == 0 ? 64 : (p.page_size % 32 == 0 ? 32 : 16);
     a.max_pages = (int)p.max_pages;
     a.scale = p.scale;
+    a.prefix = reinterpret_cast<int64_t*>(a.parts + (int64_t)a.row_tiles * a.groups * 2 * kRows * (kValue + 1));
     DecodeMaps maps;
     const cuuint64_t qdims[3] = {(cuuint64_t)kWidth, (cuuint64_t)a.R, (cuuint64_t)p.B};
     const cuuint64_t qstrides[2] = {(cuuint64_t)p.q_stride[1] * 2, (cuuint64_t)p.q_stride[0] * 2};
@@ -468,11 +552,13 @@ int launch_latent_decode(const fkda_latent_decode_params& p, cudaStream_t stream
     if (!encode_bf16_map(&maps.q, 3, p.q, qdims, qstrides, qbox) || !encode_bf16_map(&maps.cache, 3, p.cache, cdims, cstrides, cbox))
         return FKDA_ERR_LAUNCH;
     const int ctas = a.row_tiles * a.groups;
-    const int64_t joins = p.B * ((a.R + 7) / 8);
+    // rows of a joining CTA: one, or more where there are more rows than would be joined at once
+    const int rows_each = (int)std::min<int64_t>(8, std::max<int64_t>(1, p.B * a.R / (2 * device_sm_count())));
+    const int64_t joins = p.B * ((a.R + rows_each - 1) / rows_each);
     if (joins > 0x7fffffff) return FKDA_ERR_BAD_SHAPE;
     if (!allow_smem<latent_decode_kernel>(kSmem)) return FKDA_ERR_LAUNCH;
     if (!launch_dependent(latent_decode_kernel, ctas, kThreads, kSmem, stream, a, maps)) return FKDA_ERR_LAUNCH;
-    if (!launch_dependent(latent_join_kernel, joins, 256, 0, stream, a, ctas)) return FKDA_ERR_LAUNCH;
+    if (!launch_dependent(latent_join_kernel, joins, 128 * kJoinGroups, 0, stream, a, ctas, rows_each)) return FKDA_ERR_LAUNCH;
     *n_launches = 2;
     return FKDA_OK;
 }

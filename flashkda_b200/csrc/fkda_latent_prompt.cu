@@ -12,6 +12,7 @@
 // Numerics: products of bf16 with fp32 sums, weights relative to a reference that follows the running maximum once that is
 // 2^8 above it (so weights stay below 2^8 and the sums are exact to 32 bits either way), weights rounded to bf16 for the product
 // with v (their relative error, 2^-9 at most, averages out over the keys; the sum and lse use the unrounded weights).
+#define FKDA_WAITS_INLINE
 #include "fkda_tc5.cuh"
 
 namespace fkda {
@@ -28,7 +29,7 @@ constexpr int kThreads = 384;                // two softmax warpgroups, and one 
 // Registers of a thread: 168 at launch, then 208 for a row's 128 scores and what is made of them; 2 x 208 + 88 = 3 x 168
 constexpr int kRegsRow = 208, kRegsRest = 88;
 static_assert(2 * kRegsRow + kRegsRest <= 3 * 168, "a block has no more");
-constexpr int kSmem = 1024 + (2 * kKeyTiles + kSlots) * kSlotBytes + 256;
+constexpr int kSmem = (2 * kKeyTiles + kSlots) * kSlotBytes + 256;
 constexpr uint32_t kS = 0, kO = 256;         // tensor-memory columns: scores (and weights) of the two tiles, outputs
 
 struct PromptMaps {
@@ -107,12 +108,11 @@ __device__ __forceinline__ Place locate(const PromptArgs& a, int64_t slot, int l
 }
 
 __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ PromptMaps maps) {
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* q_smem = smem;                                        // [2 tiles][3][128 rows][128 bytes]
     uint8_t* ring = smem + 2 * kKeyTiles * kSlotBytes;
     Bars& bar = *reinterpret_cast<Bars*>(ring + kSlots * kSlotBytes);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         mbar_init(&bar.q_full, 1);
         for (int i = 0; i < kSlots; ++i) mbar_init(&bar.full[i], 1), mbar_init(&bar.empty[i], 1);
@@ -127,9 +127,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
     grid_dep_wait();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = bar.tmem;
-    const Place p = locate(a, blockIdx.x / a.H, lane);
-    const int h = (int)(blockIdx.x % a.H);
+    constexpr uint32_t tmem = 0;   // (all columns are this CTA's)
+    Place p = locate(a, blockIdx.x / a.H, lane);
+    p.any = p.any && as_assumed(smem, bar.tmem);
+    const int h = (int)(blockIdx.x % (uint32_t)a.H);
     // key blocks of the two tiles: a row sees the keys up to its own place counted from the ends
     int n[2] = {0, 0};
     if (p.any) {
@@ -137,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
         for (int w = 0; w < 2; ++w) {
             const int last = min(p.row0 + (w + 1) * kTile, p.len_q);   // one past the tile's last row
             const int seen = a.causal ? min(p.len_k, max(0, p.len_k - p.len_q + last)) : p.len_k;
-            n[w] = p.row0 + w * kTile < p.len_q ? (seen + kTile - 1) / kTile : 0;
+            n[w] = uniform(p.row0 + w * kTile < p.len_q ? (seen + kTile - 1) / kTile : 0);
         }
     }
     const int blocks = max(n[0], n[1]);
@@ -146,76 +147,85 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
     regs_dec<kRegsRest>();
     if (warp == 8) {
         // ---- loads: the queries, then for every block its keys (two tiles of the head's, one of the token's) and values ----
-        if (blocks > 0 && elect_one()) {
-            mbar_arrive_expect_tx(&bar.q_full, 2 * kKeyTiles * kSlotBytes);
+        if (blocks > 0) {
+            const uint32_t q_addr = smem_u32(q_smem), ring_addr = smem_u32(ring), leader = elect_one();
+            const int q0 = uniform((int)(p.q0 + p.row0)), row = uniform((int)p.b), k0 = uniform((int)p.k0);
+            expect(&bar.q_full, 2 * kKeyTiles * kSlotBytes, leader);
+#pragma unroll 1
             for (int w = 0; w < 2; ++w)
-                for (int c = 0; c < kKeyTiles; ++c)
-                    tma_load_4d(q_smem + (w * kKeyTiles + c) * kSlotBytes, &maps.q, c * 64, h, (int)(p.q0 + p.row0 + w * kTile), (int)p.b, &bar.q_full);
+#pragma unroll
+                for (int c = 0; c < kKeyTiles; ++c) load_4d(q_addr + (w * kKeyTiles + c) * kSlotBytes, &maps.q, c * 64, h, q0 + w * kTile, row, &bar.q_full, leader);
             int s = 0;
             bool ok = true;
+#pragma unroll 1
             for (int i = 0; i < blocks && ok; ++i) {
-                const int t = (int)p.k0 + i * kTile;
-                for (int c = 0; c < kKeyTiles + kValueTiles && ok; ++c, ++s) {
+                const int t = k0 + i * kTile;
+#pragma unroll
+                for (int c = 0; c < kKeyTiles + kValueTiles; ++c, ++s) {
                     const int slot = s % kSlots;
-                    if (s >= kSlots) ok = wait(&bar.empty[slot], (s / kSlots - 1) & 1, &bar.abort);
+                    if (s >= kSlots) ok = __all_sync(0xffffffffu, wait(&bar.empty[slot], (s / kSlots - 1) & 1, &bar.abort));
                     if (!ok) break;
-                    uint8_t* dst = ring + slot * kSlotBytes;
-                    mbar_arrive_expect_tx(&bar.full[slot], kSlotBytes);
-                    if (c < 2) tma_load_4d(dst, &maps.k, c * 64, h, t, (int)p.b, &bar.full[slot]);
-                    else if (c == 2) tma_load_3d(dst, &maps.r, 0, t, (int)p.b, &bar.full[slot]);
-                    else tma_load_4d(dst, &maps.v, (c - 3) * 64, h, t, (int)p.b, &bar.full[slot]);
+                    const uint32_t dst = ring_addr + slot * kSlotBytes;
+                    expect(&bar.full[slot], kSlotBytes, leader);
+                    if (c < 2) load_4d(dst, &maps.k, c * 64, h, t, row, &bar.full[slot], leader);
+                    else if (c == 2) load_3d(dst, &maps.r, 0, t, row, &bar.full[slot], leader);
+                    else load_4d(dst, &maps.v, (c - 3) * 64, h, t, row, &bar.full[slot], leader);
                 }
             }
             drain(&bar.q_full, 0);
+#pragma unroll 1
             for (int k = max(0, s - kSlots); k < s; ++k) drain(&bar.full[k % kSlots], (k / kSlots) & 1);
+            __syncwarp();
         }
     } else if (warp == 9) {
         // ---- products ----
-        if (blocks > 0 && elect_one()) {
+        if (blocks > 0) {
             constexpr uint32_t kIdS = idesc(kTile, kTile, false, false), kIdO = idesc(kTile, 64, false, true);
-            const uint32_t q_addr = smem_u32(q_smem), ring_addr = smem_u32(ring);
+            const uint32_t q_desc = desc(smem_u32(q_smem)), ring_desc = desc(smem_u32(ring)), leader = elect_one();
             constexpr int kEach = kKeyTiles + kValueTiles;
-            bool ok = wait(&bar.q_full, 0, &bar.abort);
+            wait_warp(&bar.q_full, 0, &bar.abort);
             auto scores = [&](int w, int i, bool first) {   // tile w against key block i
+#pragma unroll
                 for (int c = 0; c < kKeyTiles; ++c) {
                     const int s = i * kEach + c;
-                    if (first && ok) ok = wait(&bar.full[s % kSlots], (s / kSlots) & 1, &bar.abort);
+                    if (first) wait_warp(&bar.full[s % kSlots], (s / kSlots) & 1, &bar.abort);
                     fence_after();
+                    const uint32_t k_desc = ring_desc + (s % kSlots) * (kSlotBytes / 16);
+#pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        mma_ss(tmem + kS + w * kTile, desc(q_addr + (w * kKeyTiles + c) * kSlotBytes + k * 32),
-                               desc(ring_addr + (s % kSlots) * kSlotBytes + k * 32), kIdS, (c | k) != 0);
+                        mma_ss(tmem + kS + w * kTile, q_desc + ((w * kKeyTiles + c) * kSlotBytes + k * 32) / 16, k_desc + k * 32 / 16, kIdS, (c | k) != 0, leader);
                 }
-                commit(&bar.s_full[w]);
+                commit(&bar.s_full[w], leader);
             };
             auto free_slots = [&](int first, int count) {
-                for (int s = first; s < first + count; ++s) commit(&bar.empty[s % kSlots]);
+                for (int s = first; s < first + count; ++s) commit(&bar.empty[s % kSlots], leader);
             };
 #pragma unroll
             for (int w = 0; w < 2; ++w)
-                if (n[w] > 0 && ok) scores(w, 0, w == 0 || n[0] == 0);
+                if (n[w] > 0) scores(w, 0, w == 0 || n[0] == 0);
             free_slots(0, kKeyTiles);
-            for (int i = 0; i < blocks && ok; ++i) {
+#pragma unroll 1
+            for (int i = 0; i < blocks; ++i) {
                 const int first_v = i < n[0] ? 0 : 1, last_v = i < n[1] ? 1 : 0;
                 const int first_k = i + 1 < n[0] ? 0 : 1, last_k = i + 1 < n[1] ? 1 : 0;
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
-                    if (i >= n[w] || !ok) continue;
-                    for (int half = 0; half < 2 && ok; ++half) {   // 64 keys
-                        ok = wait(&bar.p_full[w][half], i & 1, &bar.abort);
-                        for (int c = 0; c < kValueTiles && half == 0 && w == first_v && ok; ++c) {
-                            const int s = i * kEach + kKeyTiles + c;
-                            ok = wait(&bar.full[s % kSlots], (s / kSlots) & 1, &bar.abort);
-                        }
-                        if (!ok) break;
+                    if (i >= n[w]) continue;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {   // 64 keys
+                        wait_warp(&bar.p_full[w][half], i & 1, &bar.abort);
+                        if (half == 0 && w == first_v)
+                            for (int s = i * kEach + kKeyTiles; s < (i + 1) * kEach; ++s) wait_warp(&bar.full[s % kSlots], (s / kSlots) & 1, &bar.abort);
                         fence_after();
+#pragma unroll
                         for (int c = 0; c < kValueTiles; ++c) {   // 64 dimensions at a time: the two tiles need not be neighbours in the ring
-                            const uint32_t v_addr = ring_addr + ((i * kEach + kKeyTiles + c) % kSlots) * kSlotBytes;
+                            const uint32_t v_desc = ring_desc + ((i * kEach + kKeyTiles + c) % kSlots) * (kSlotBytes / 16);
+#pragma unroll
                             for (int k = 4 * half; k < 4 * half + 4; ++k)
-                                mma_ts(tmem + kO + w * kTile + c * 64, tmem + kS + w * kTile + k * 8, desc(v_addr + k * 2048), kIdO, i > 0 || k > 0);
+                                mma_ts(tmem + kO + w * kTile + c * 64, tmem + kS + w * kTile + k * 8, v_desc + k * 2048 / 16, kIdO, i > 0 || k > 0, leader);
                         }
                     }
-                    if (!ok) break;
-                    commit(&bar.o_done[w]);
+                    commit(&bar.o_done[w], leader);
                     if (w == last_v) free_slots(i * kEach + kKeyTiles, kValueTiles);
                     if (i + 1 < n[w]) {
                         scores(w, i + 1, w == first_k);
@@ -223,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
                     }
                 }
             }
-            commit(&bar.drained);
+            commit(&bar.drained, leader);
             drain(&bar.drained, 0);
         }
     }

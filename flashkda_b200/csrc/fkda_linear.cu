@@ -51,7 +51,7 @@ struct LinearMaps {
     CUtensorMap q, k, v, out;
 };
 struct Decays {
-    float G[kC], eG[kC], w[kC], total;
+    alignas(16) float G[kC], eG[kC], w[kC], total;
     float pad[3];
 };
 // (A barrier that one side may complete twice before the other has looked is there once per buffer.)
@@ -62,7 +62,7 @@ struct Bars {
     uint32_t tmem;
     int abort;
 };
-constexpr int kSmem = 1024 + kOffBars + ((int)sizeof(Bars) + 127) / 128 * 128;
+constexpr int kSmem = kOffBars + ((int)sizeof(Bars) + 127) / 128 * 128;
 static_assert(kSmem <= 232448, "shared memory of an SM");
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -131,10 +131,9 @@ __device__ __forceinline__ void store_state32(const LinearArgs& a, int64_t at, c
 }
 
 __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_constant__ LinearArgs a, const __grid_constant__ LinearMaps maps) {
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    extern __shared__ __align__(1024) uint8_t smem[];
     Bars& bar = *reinterpret_cast<Bars*>(smem + kOffBars);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) mbar_init(&bar.full[i], 1), mbar_init(&bar.empty[i], 2), mbar_init(&bar.dec_full[i], 1), mbar_init(&bar.dec_empty[i], 24);
         for (int i = 0; i < 2; ++i) mbar_init(&bar.p_full[i], 128), mbar_init(&bar.p_free[i], 1), mbar_init(&bar.w_full[i], 128);
@@ -154,105 +153,106 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     grid_dep_wait();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = bar.tmem;
+    constexpr uint32_t tmem = 0;   // (all columns are this CTA's)
     const Chain ch = locate(a, blockIdx.x);
-    const bool mine = !(a.skip_single && ch.len <= 1);
-    const int n = mine ? (ch.len + kC - 1) / kC : 0;
+    const bool mine = !(a.skip_single && ch.len <= 1) && as_assumed(smem, bar.tmem);
+    const int n = uniform(mine ? (ch.len + kC - 1) / kC : 0);
 
     if (warp == 24) {
         // ---- copies ----
-        if (elect_one()) {
-            bool ok = true;
-            int c = 0;
+        const uint32_t base = smem_u32(smem), leader = elect_one();
+        const int t0 = uniform((int)ch.t0), row = uniform((int)ch.b), head = uniform(ch.h), key_head = uniform(ch.h / a.group);
+        int c = 0, stage = 0, phase = 1;
 #pragma unroll 1
-            for (; c < n; ++c) {
-                const int s = c % kStages;
-                if (c >= kStages) ok = wait(&bar.empty[s], (c / kStages - 1) & 1, &bar.abort);
-                if (!ok) break;
-                uint8_t* dst = smem + s * kStageBytes;
-                const int t = (int)ch.t0 + c * kC;
-                mbar_arrive_expect_tx(&bar.full[s], kStageBytes);
-                for (int x = 0; x < 2; ++x) {
-                    tma_load_4d(dst + x * kTileBytes, &maps.q, x * 64, ch.h / a.group, t, (int)ch.b, &bar.full[s]);
-                    tma_load_4d(dst + kOperandBytes + x * kTileBytes, &maps.k, x * 64, ch.h / a.group, t, (int)ch.b, &bar.full[s]);
-                    tma_load_4d(dst + 2 * kOperandBytes + x * kTileBytes, &maps.v, x * 64, ch.h, t, (int)ch.b, &bar.full[s]);
-                }
+        for (; c < n; ++c) {
+            if (c >= kStages && !__all_sync(0xffffffffu, wait(&bar.empty[stage], phase, &bar.abort))) break;
+            const uint32_t dst = base + stage * kStageBytes;
+            expect(&bar.full[stage], kStageBytes, leader);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                load_4d(dst + x * kTileBytes, &maps.q, x * 64, key_head, t0 + c * kC, row, &bar.full[stage], leader);
+                load_4d(dst + kOperandBytes + x * kTileBytes, &maps.k, x * 64, key_head, t0 + c * kC, row, &bar.full[stage], leader);
+                load_4d(dst + 2 * kOperandBytes + x * kTileBytes, &maps.v, x * 64, head, t0 + c * kC, row, &bar.full[stage], leader);
             }
-            for (int k = max(0, c - kStages); k < c; ++k) drain(&bar.full[k % kStages], (k / kStages) & 1);
+            if (++stage == kStages) stage = 0, phase ^= 1;
         }
+#pragma unroll 1
+        for (int k = max(0, c - kStages); k < c; ++k) drain(&bar.full[k % kStages], (k / kStages) & 1);
+        __syncwarp();
     } else if (warp == 25) {
         // ---- products of the state, which the next chunk waits for, and scores ----
-        if (n > 0 && elect_one()) {
-            const uint32_t base = smem_u32(smem);
+        if (n > 0) {
+            const uint32_t base = smem_u32(smem), leader = elect_one();
             constexpr uint32_t kIdScore = idesc(64, 64, false, false), kIdState = idesc(128, 64, false, true);
-            bool ok = true;
-            auto until = [&](uint64_t* b, int phase) { ok = ok && wait(b, phase & 1, &bar.abort); };
-            auto score = [&](int c) {
-                until(&bar.full[c % kStages], c / kStages);
-                if (c > 0) until(&bar.score_free, c - 1);
-                if (!ok) return;
-                fence_after();
-                const uint32_t q = base + (c % kStages) * kStageBytes, k = q + kOperandBytes;
-                for (int x = 0; x < 2; ++x)
-                    for (int i = 0; i < 4; ++i)
-                        mma_ss(tmem + kScore, desc(q + x * kTileBytes + i * 32), desc(k + x * kTileBytes + i * 32), kIdScore, (x | i) != 0);
-                commit(&bar.score);
-            };
-            score(0);
+            int stage = 0, phase = 0;   // of the chunk whose scores are next
+            uint32_t k = 0;             // keys of the chunk in front of it
 #pragma unroll 1
-            for (int c = 0; c < n && ok; ++c) {
-                const uint32_t k = base + (c % kStages) * kStageBytes + kOperandBytes;
+            for (int c = -1; c < n; ++c) {
+                if (c >= 0) {
 #pragma unroll 1
-                for (int h = 0; h < 2; ++h) {   // 64 columns of the state, while the other 64 are being decayed
-                    until(&bar.scaled[h], c);
-                    for (int half = 0; half < 2; ++half) {
-                        if (h == 0) until(&bar.w_full[half], c);
-                        if (!ok) break;
+                    for (int h = 0; h < 2; ++h) {   // 64 columns of the state, while the other 64 are being decayed
+                        wait_warp(&bar.scaled[h], c & 1, &bar.abort);
+                        wait_warp(&bar.w_full[0], c & 1, &bar.abort);
+                        wait_warp(&bar.w_full[1], c & 1, &bar.abort);
                         fence_after();
-                        for (int i = 2 * half; i < 2 * half + 2; ++i)
+#pragma unroll 1
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
                             for (int t = 0; t < kTerms; ++t)
-                                mma_ts(tmem + kS + h * 64, tmem + kW + t * 32 + i * 8, desc(k + h * kTileBytes + i * 2048), kIdState, 1);
+                                mma_ts(tmem + kS + h * 64, tmem + kW + t * 32 + i * 8, k + h * (kTileBytes / 16) + i * (2048 / 16), kIdState, 1, leader);
+                        commit(&bar.s_done[h], leader);
                     }
-                    if (!ok) break;
-                    commit(&bar.s_done[h]);
+                    commit(&bar.empty[stage == 0 ? kStages - 1 : stage - 1], leader);
                 }
-                if (!ok) break;
-                commit(&bar.empty[c % kStages]);
-                if (c + 1 < n) score(c + 1);
+                if (c + 1 < n) {
+                    wait_warp(&bar.full[stage], phase, &bar.abort);
+                    if (c >= 0) wait_warp(&bar.score_free, c & 1, &bar.abort);
+                    fence_after();
+                    const uint32_t q = desc(base + stage * kStageBytes);
+                    k = desc(base + stage * kStageBytes + kOperandBytes);
+#pragma unroll 1
+                    for (int x = 0; x < 2; ++x)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            mma_ss(tmem + kScore, q + x * (kTileBytes / 16) + i * 2, k + x * (kTileBytes / 16) + i * 2, kIdScore, (x | i) != 0, leader);
+                    commit(&bar.score, leader);
+                    if (++stage == kStages) stage = 0, phase ^= 1;
+                }
             }
-            commit(&bar.drained[0]);
+            commit(&bar.drained[0], leader);
             drain(&bar.drained[0], 0);
         }
     } else if (warp == 27) {
         // ---- products of the outputs ----
-        if (n > 0 && elect_one()) {
-            const uint32_t base = smem_u32(smem), p_addr = base + kOffP;
+        if (n > 0) {
+            const uint32_t base = smem_u32(smem), leader = elect_one();
             constexpr uint32_t kIdO1 = idesc(128, 64, false, false), kIdO2 = idesc(128, 64, true, false);
-            bool ok = true;
-            auto until = [&](uint64_t* b, int phase) { ok = ok && wait(b, phase & 1, &bar.abort); };
+            int stage = 0, phase = 0;
 #pragma unroll 1
             for (int c = 0; c < n; ++c) {
-                const uint32_t q = base + (c % kStages) * kStageBytes, v = q + 2 * kOperandBytes;
-                until(&bar.full[c % kStages], c / kStages);
-                until(&bar.scaled[1], c);   // (the copy is there as well)
-                if (c > 0) until(&bar.out_free, c - 1);
-                if (!ok) break;
+                const uint32_t q = desc(base + stage * kStageBytes), v = desc(base + stage * kStageBytes + 2 * kOperandBytes, kTileBytes);
+                wait_warp(&bar.full[stage], phase, &bar.abort);
+                wait_warp(&bar.scaled[1], c & 1, &bar.abort);   // (the copy is there as well)
+                if (c > 0) wait_warp(&bar.out_free, (c - 1) & 1, &bar.abort);
                 fence_after();
+#pragma unroll 1
                 for (int x = 0; x < 2; ++x)
+#pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        mma_ts(tmem + kO1, tmem + kCopy + x * 32 + i * 8, desc(q + x * kTileBytes + i * 32), kIdO1, (x | i) != 0);
-                commit(&bar.copy_free);
-                if (c + 1 == n) until(&bar.w_full[1], c);   // (values behind the sequence's end are nothing by now)
-                until(&bar.p_full[c & 1], c >> 1);
-                if (!ok) break;
+                        mma_ts(tmem + kO1, tmem + kCopy + x * 32 + i * 8, q + (x * kTileBytes + i * 32) / 16, kIdO1, (x | i) != 0, leader);
+                commit(&bar.copy_free, leader);
+                if (c + 1 == n) wait_warp(&bar.w_full[1], c & 1, &bar.abort);   // (values behind the sequence's end are nothing by now)
+                wait_warp(&bar.p_full[c & 1], (c >> 1) & 1, &bar.abort);
                 fence_after();
-                for (int i = 0; i < 4; ++i)
-                    mma_ss(tmem + kO2, desc(v + i * 2048, kTileBytes), desc(p_addr + (c & 1) * kTileBytes + i * 32), kIdO2, i != 0);
-                commit(&bar.p_free[c & 1]);
-                commit(&bar.out_full);
-                commit(&bar.empty[c % kStages]);
+                const uint32_t p = desc(base + kOffP + (c & 1) * kTileBytes);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mma_ss(tmem + kO2, v + i * 2048 / 16, p + i * 32 / 16, kIdO2, i != 0, leader);
+                commit(&bar.p_free[c & 1], leader);
+                commit(&bar.out_full, leader);
+                commit(&bar.empty[stage], leader);
+                if (++stage == kStages) stage = 0, phase ^= 1;
             }
-            commit(&bar.drained[1]);
+            commit(&bar.drained[1], leader);
             drain(&bar.drained[1], 0);
         }
     } else if (warp == 26) {
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
             const int t = c * kC + 2 * lane;
             const float x = t < ch.len ? log2_decay(g[t * a.g_token]) : 0.0f, y = t + 1 < ch.len ? log2_decay(g[(t + 1) * a.g_token]) : 0.0f;
             float upto = x + y, from = x + y;   // sums over the lanes up to mine, and from mine on
-#pragma unroll
+#pragma unroll 1
             for (int off = 1; off < 32; off <<= 1) {
                 const float p = __shfl_up_sync(0xffffffffu, upto, off), q = __shfl_down_sync(0xffffffffu, from, off);
                 if (lane >= off) upto += p;

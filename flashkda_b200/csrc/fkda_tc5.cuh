@@ -13,14 +13,21 @@ using namespace sm100;
 
 // ------------------------------------------------------------------ waits ----
 // Every wait of these kernels is bounded.  One that gives up raises the CTA's abort flag, at which the other waits of the CTA
-// return at once: the roles run to their ends on whatever is in shared memory (all accesses in bounds), the copies and
-// products in flight are waited for, tensor memory is freed, and the word below tells the host (fkda_operator_status).
+// return at once: copies end, the other roles run to their ends on whatever is in shared memory (all accesses in bounds), what is
+// in flight is waited for, tensor memory is freed, and the word below tells the host (fkda_operator_status).
 static __device__ int32_t g_gave_up = 0;
 // The limit is counted in SM cycles (two seconds at 2 GHz): the global timer is far away, and reading it in the waits of a dozen
 // warps made all of them slower.
 constexpr long long kWaitCycles = 4000000000ll;
 
-__device__ __forceinline__ bool wait_until(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+// Not inlined: thirty copies of it leave the roles' loops less room in the instruction cache.  (Except where a role takes nearly all
+// registers that a thread can have: a call has its own there.)
+#ifdef FKDA_WAITS_INLINE
+#define FKDA_WAIT_INLINE __forceinline__
+#else
+#define FKDA_WAIT_INLINE __noinline__
+#endif
+static __device__ FKDA_WAIT_INLINE bool wait_on(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
     long long start = 0;
     for (uint32_t spins = 0; !mbar_try_wait(bar, parity); ++spins) {
         if ((spins & 31u) != 31u) continue;
@@ -30,6 +37,9 @@ __device__ __forceinline__ bool wait_until(uint64_t* bar, uint32_t parity, volat
         if (now - start > kWaitCycles) return false;
     }
     return true;
+}
+__device__ __forceinline__ bool wait_until(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    return mbar_try_wait(bar, parity) || wait_on(bar, parity, abort_flag);
 }
 
 // The word of this translation unit's kernels, once the stream has come this far; cleared for the next reader.
@@ -42,11 +52,13 @@ static int read_gave_up(cudaStream_t stream, int32_t* word) {
     return FKDA_OK;
 }
 
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* abort_flag) {
-    if (wait_until(bar, parity, abort_flag)) return true;
+static __device__ FKDA_WAIT_INLINE bool give_up(int* abort_flag) {
     *reinterpret_cast<volatile int*>(abort_flag) = 1;
     g_gave_up = 1;
     return false;
+}
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* abort_flag) {
+    return wait_until(bar, parity, abort_flag) || give_up(abort_flag);
 }
 // The same for a whole warp, whose lanes leave it together: what follows may be an access to tensor memory or another instruction that
 // a warp executes as one.
@@ -75,13 +87,30 @@ __device__ __forceinline__ bool named_any(int id, int threads, bool x) {
     return any != 0;
 }
 
-__device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* tmap, int c0, int c1, int c2, int c3, uint64_t* bar) {
+// Copies are issued by the lane with `leader` = 1 of a warp that runs the code around them as a whole, as products are (below).
+__device__ __forceinline__ void expect(uint64_t* bar, uint32_t bytes, uint32_t leader) {
+    asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %2, 0;\n@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}\n" ::"r"(smem_u32(bar)), "r"(bytes), "r"(leader) : "memory");
+}
+__device__ __forceinline__ void load_4d(uint32_t dst, const void* tmap, int c0, int c1, int c2, int c3, uint64_t* bar, uint32_t leader) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-        ::"r"(smem_u32(smem_dst)), "l"(tmap), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+        "{\n.reg .pred q;\nsetp.ne.b32 q, %7, 0;\n"
+        "@q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n}\n" ::"r"(dst), "l"(tmap),
+        "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar)), "r"(leader)
         : "memory");
 }
-
+__device__ __forceinline__ void load_3d(uint32_t dst, const void* tmap, int c0, int c1, int c2, uint64_t* bar, uint32_t leader) {
+    asm volatile(
+        "{\n.reg .pred q;\nsetp.ne.b32 q, %6, 0;\n"
+        "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n}\n" ::"r"(dst), "l"(tmap),
+        "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar)), "r"(leader)
+        : "memory");
+}
+// The same tile into L2 only, ahead of its load.
+__device__ __forceinline__ void prefetch_3d(const void* tmap, int c0, int c1, int c2, uint32_t leader) {
+    asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %4, 0;\n@q cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];\n}\n" ::"l"(tmap), "r"(c0), "r"(c1), "r"(c2),
+                 "r"(leader)
+                 : "memory");
+}
 __device__ __forceinline__ void tma_store_4d(const void* tmap, int c0, int c1, int c2, int c3, const void* smem_src) {
     asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(tmap), "r"(c0), "r"(c1), "r"(c2),
                  "r"(c3), "r"(smem_u32(smem_src))
@@ -169,6 +198,14 @@ __device__ __forceinline__ void st_frag8(uint32_t taddr, uint32_t r0, uint32_t r
     asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
 }
 
+// The kernels count on dynamic shared memory that starts at a multiple of 1024 bytes, as it is declared, and on tensor memory that starts
+// at 0 where a CTA has all of it: then addresses and descriptors are constants.  (Never seen otherwise; checked all the same.)
+__device__ __forceinline__ bool as_assumed(const void* smem, uint32_t tmem) {
+    if ((smem_u32(smem) & 1023u) == 0 && tmem == 0) return true;
+    g_gave_up = 1;
+    return false;
+}
+
 // A warpgroup's registers per thread from here on: `inc` waits until others have given up as many (the shares of all warpgroups of a
 // block may not add up to more than it was launched with).
 template <int N>
@@ -202,32 +239,38 @@ __device__ __forceinline__ void sub2(uint32_t& x, uint32_t& y, uint32_t bx, uint
 //   MN-major operand: a tile row is one step of K, the tile's columns are 64 rows (M or N) of the operand; 16 steps are 2048 bytes
 //     of the start address; `block` is the distance to the tile of the next 64 rows.
 // Fields: start address [0,14), leading distance [16,30), stride of 8-row groups [32,46) (all >> 4), version 1 at bit 46,
-// swizzle mode 2 (128 bytes) at [61,64).
-__device__ __forceinline__ uint64_t desc(uint32_t smem_addr, uint32_t block = 16) {
-    return (uint64_t)((smem_addr >> 4) & 0x3fffu) | (uint64_t)((block >> 4) & 0x3fffu) << 16 | (uint64_t)(1024 >> 4) << 32 |
-           (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
+// swizzle mode 2 (128 bytes) at [61,64).  The upper word is the same for all; this is the lower one.
+constexpr uint32_t kDescUpper = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc(uint32_t smem_addr, uint32_t block = 16) { return ((smem_addr >> 4) & 0x3fffu) | ((block >> 4) << 16); }
 // Instruction descriptor for bf16 operands and fp32 accumulation: D format [4,6) = 1, A and B formats [7,10), [10,13) = 1, MN-major
 // flags of A and B at bits 15 and 16, N >> 3 at [17,23), M >> 4 at [24,29).
 __host__ __device__ constexpr uint32_t idesc(int M, int N, bool a_mn, bool b_mn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
            ((uint32_t)(M >> 4) << 24);
 }
-// D[tmem] (+)= A[smem] B[smem], K = 16; issued by ONE thread.  accumulate = 0 overwrites D.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-                 "l"(a), "l"(b), "r"(id), "r"(accumulate)
-                 : "memory");
+// Products are issued by ONE thread, but a whole warp runs the code around them, with the same values in all lanes: then descriptors are
+// uniform registers, and an instruction goes out every 32 to 64 cycles (what its operands take) instead of every 75 (A in tensor memory)
+// or 116.  `leader` is 1 in the lane that issues.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+// D[tmem] (+)= A[smem] B[smem], K = 16; accumulate = 0 overwrites D.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t accumulate, uint32_t leader) {
+    asm volatile(
+        "{\n.reg .pred p, q;\n.reg .b64 da, db;\nmov.b64 da, {%1, %5};\nmov.b64 db, {%2, %5};\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %6, 0;\n"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(id), "r"(accumulate), "r"(kDescUpper), "r"(leader)
+        : "memory");
 }
 // D[tmem] (+)= A[tmem] B[smem]: A sits in tensor memory, two bf16 per 32-bit column (8 columns per instruction).
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-                 "r"(a), "l"(b), "r"(id), "r"(accumulate)
-                 : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t accumulate, uint32_t leader) {
+    asm volatile(
+        "{\n.reg .pred p, q;\n.reg .b64 db;\nmov.b64 db, {%2, %5};\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %6, 0;\n"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(id), "r"(accumulate), "r"(kDescUpper), "r"(leader)
+        : "memory");
 }
-// The mbarrier completes when all tcgen05.mma issued so far by this thread have.
-__device__ __forceinline__ void commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+// The mbarrier completes when all tcgen05.mma issued so far by the leader have.
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t leader) {
+    asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %1, 0;\n@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
+                 "r"(leader)
+                 : "memory");
 }
 
 __device__ __forceinline__ float f(uint32_t x) { return __uint_as_float(x); }
