@@ -16,7 +16,9 @@
 // Numerics: as in the expanded form (fp32 scores, sums and outputs; weights against a reference within 2^8 of the running maximum,
 // rounded to bf16 for the value product only); parts are joined in fp32 in the order of the tokens.
 #include <algorithm>
+#include <type_traits>
 
+#define FKDA_WAITS_INLINE
 #include "fkda_tc5.cuh"
 
 namespace fkda {
@@ -42,7 +44,7 @@ struct DecodeArgs {
     const __nv_bfloat16* cache;
     int64_t page_stride;     // elements from page to page where a page's tokens lie one behind the other, else 0 (no fetching ahead)
     float* parts;        // [CTAs][2][kRows][kValue], then their lse [CTAs][2][kRows]
-    int64_t* prefix;     // [B + 1] tiles in front of each sequence, and of all
+    int4* spans;         // [B] first and last group of CTAs with tiles of a sequence, whether the first begins with it
     int64_t out_batch, out_row, table_stride, pages;
     int B, Tq, H, R, row_tiles, groups, page, box, max_pages;
     float scale;
@@ -128,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
         const int64_t share = (total + a.groups - 1) / a.groups, mine = share * group;
         int64_t seen = 0;
-        for (int base = 0; base < a.B; base += 32) {
+        for (int base = 0, turn = 0; base < a.B; base += 32, turn = turn + 1 == a.groups ? 0 : turn + 1) {
             const int c = base + lane < a.B ? counts[base + lane] : 0;
             int upto = c;
 #pragma unroll
@@ -142,10 +144,23 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
                 bar.first_tile = (int)(mine - before);
                 bar.count = (int)min(share, total - mine);
             }
-            if (blockIdx.x == 0 && base + lane < a.B) a.prefix[base + lane] = before;
+            if (rt == 0 && turn == group && base + lane < a.B) {   // (the groups note 32 sequences each in turn)
+                const int first = c > 0 ? (int)(before / share) : 0, last = c > 0 ? (int)((before + c - 1) / share) : 0;
+                a.spans[base + lane] = make_int4(first, last, first * share == before ? 1 : 0, 0);
+            }
             seen += __shfl_sync(0xffffffffu, upto, 31);
         }
-        if (blockIdx.x == 0 && lane == 0) a.prefix[a.B] = total;
+    } else if (warp < 4) {
+        // sequences without any token: nothing
+        for (int b = group; b < a.B; b += a.groups) {
+            if (counts[b] != 0) continue;
+            for (int i = threadIdx.x - 32; i < kRows * (kValue / 8); i += 96) {
+                const int row = rt * kRows + i / (kValue / 8);
+                if (row >= a.R) break;
+                *reinterpret_cast<uint4*>(a.out + (int64_t)b * a.out_batch + (int64_t)row * a.out_row + i % (kValue / 8) * 8) = make_uint4(0, 0, 0, 0);
+                if (i % (kValue / 8) == 0 && a.lse != nullptr) a.lse[(int64_t)b * a.R + row] = -INFINITY;
+            }
+        }
     }
     fence_proxy_async_smem();   // (the stages are written by copies from here on)
     __syncthreads();
@@ -173,13 +188,6 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         for (; ok && walk.next(a); walk.done(), ++pieces) {
             fetch_ahead(walk.t + 1);
             __syncwarp();
-            if (pieces > 0) ok = __all_sync(0xffffffffu, wait(&bar.q_empty, (pieces - 1) & 1, &bar.abort));
-            if (!ok) break;
-            expect(&bar.q_full, kStageBytes, leader);
-            ++asked;
-            const int seq = uniform(walk.b);
-#pragma unroll 1
-            for (int c = 0; c < kChunks; ++c) load_3d(q_addr + c * kChunkBytes, &maps.q, c * 64, rt * kRows, seq, &bar.q_full, leader);
 #pragma unroll 1
             for (int t = walk.t; t < walk.until; ++t, ++g) {
                 const int tok = t * kTok + lane * a.box;
@@ -204,6 +212,15 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
                     issued = g * kGroups + j + 1;
                 }
                 if (!ok) break;
+                if (t > walk.t) continue;
+                // the stretch's queries, once the last one's have been read
+                if (pieces > 0) ok = __all_sync(0xffffffffu, wait(&bar.q_empty, (pieces - 1) & 1, &bar.abort));
+                if (!ok) break;
+                expect(&bar.q_full, kStageBytes, leader);
+                ++asked;
+                const int seq = uniform(walk.b);
+#pragma unroll 1
+                for (int c = 0; c < kChunks; ++c) load_3d(q_addr + c * kChunkBytes, &maps.q, c * 64, rt * kRows, seq, &bar.q_full, leader);
             }
             if (!ok) break;
         }
@@ -214,9 +231,32 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     } else if (warp == 5) {
         // ---- products: two lines of work, each taken up as soon as what it waits for is there: the scores of tile `g`, group by group of its
         //      dimensions, at most one tile ahead of the value product of tile `done` ----
-        constexpr uint32_t kIdS = idesc(kRows, kTok, false, false), kIdO = idesc(128, kRows, true, false);
         const uint32_t q_desc = desc(smem_u32(q_smem)), k_desc = desc(smem_u32(stages)), leader = elect_one();
         const uint32_t v_desc = desc(smem_u32(stages), kChunkBytes), p_desc = desc(smem_u32(p_smem));
+        // the groups that are there, from the next one on (stage and group in the code, so that the operands are constants)
+        auto scores = [q_desc, k_desc, leader](auto stage, uint32_t there, int& group) {
+            constexpr int kStage = decltype(stage)::value;
+#pragma unroll
+            for (int j = 0; j < kGroups; ++j) {
+                if (group != j || (there >> j & 1) == 0) continue;
+#pragma unroll
+                for (int i = 8 * j; i < min(8 * j + 8, 4 * kChunks); ++i) {
+                    const int at = (i / 4 * kChunkBytes + i % 4 * 32) / 16;
+                    mma_ss(kS + kStage * kTok, q_desc + at, k_desc + kStage * (kStageBytes / 16) + at, idesc(kRows, kTok, false, false), i != 0, leader);
+                }
+                ++group;
+            }
+        };
+        auto values = [v_desc, p_desc, leader, &bar](auto stage, uint32_t adds) {
+            constexpr int kStage = decltype(stage)::value;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    mma_ss(kO + m * kRows, v_desc + (kStage * kStageBytes + 2 * m * kChunkBytes + k * 2048) / 16, p_desc + k * 32 / 16, idesc(128, kRows, true, false), k > 0 ? 1 : adds, leader);
+                commit(&bar.empty[kStage][m], leader);
+            }
+        };
         int g = 0, group_of = 0, done = 0, piece = 0;
         bool more = walk.next(a), fresh = true;           // `fresh`: the next scores are a stretch's first
         int start = walk.t;
@@ -228,19 +268,21 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
             uint64_t* look = lane < kGroups ? &bar.full[g & 1][lane] : (lane == 5 ? &bar.p_full : &bar.q_full);
             const int phase = lane < kGroups ? g >> 1 : (lane == 5 ? done : piece);
             const uint32_t there = __ballot_sync(0xffffffffu, mbar_test_wait(look, phase & 1));
-            const int scored = g;   // (`there` speaks of the weights of a tile whose scores had been issued)
             bool moved = false;
+            if (done < g && (there >> 5 & 1) != 0) {
+                fence_after();
+                const uint32_t adds = (firsts >> (done & 1) & 1) ^ 1;
+                if ((done & 1) == 0) values(std::integral_constant<int, 0>{}, adds);
+                else values(std::integral_constant<int, 1>{}, adds);
+                commit(&bar.o_done, leader);
+                ++done;
+                moved = true;
+            }
             if (more && g <= done + 1 && (!fresh || group_of > 0 || (there >> 6 & 1) != 0) && (there >> group_of & 1) != 0) {
                 fence_after();
-                const uint32_t to = tmem + kS + (g & 1) * kTok, q = q_desc + group_of * (2 * kChunkBytes / 16),
-                               k_ = k_desc + (g & 1) * (kStageBytes / 16) + group_of * (2 * kChunkBytes / 16);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) mma_ss(to, q + k * 32 / 16, k_ + k * 32 / 16, kIdS, (group_of | k) != 0, leader);
-                if (group_of < kGroups - 1) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) mma_ss(to, q + (kChunkBytes + k * 32) / 16, k_ + (kChunkBytes + k * 32) / 16, kIdS, 1, leader);
-                    ++group_of;
-                } else {
+                if ((g & 1) == 0) scores(std::integral_constant<int, 0>{}, there, group_of);
+                else scores(std::integral_constant<int, 1>{}, there, group_of);
+                if (group_of == kGroups) {
                     commit(&bar.s_full[g & 1], leader);
                     commit(&bar.empty[g & 1][kGroups - 1], leader);
                     firsts = (firsts & ~(1u << (g & 1))) | (uint32_t)fresh << (g & 1);
@@ -256,20 +298,6 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
                         ++piece;
                     }
                 }
-                moved = true;
-            }
-            if (done < scored && (there >> 5 & 1) != 0) {
-                fence_after();
-                const uint32_t v = v_desc + (done & 1) * (kStageBytes / 16), adds = (firsts >> (done & 1) & 1) ^ 1;
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        mma_ss(tmem + kO + m * kRows, v + (2 * m * kChunkBytes + k * 2048) / 16, p_desc + k * 32 / 16, kIdO, k > 0 ? 1 : adds, leader);
-                    commit(&bar.empty[done & 1][m], leader);
-                }
-                commit(&bar.o_done, leader);
-                ++done;
                 moved = true;
             }
             if (moved) {
@@ -447,62 +475,70 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     if (warp == 5) tmem_dealloc(tmem, 512);
 }
 
-// Joins the parts of the sequences that a cut runs through, and writes those without any token.  A CTA has some rows of a sequence and
-// eight groups of 128 threads, with four dimensions each: as many groups share a row, taking its parts in turn, as there are parts.
-constexpr int kJoinGroups = 8;
-__global__ void __launch_bounds__(128 * kJoinGroups) latent_join_kernel(const __grid_constant__ DecodeArgs a, int ctas, int rows_each) {
-    __shared__ float4 sums[kJoinGroups][128];
+// Joins the parts of the sequences that a cut runs through: sum of w_p O_p over the parts, w_p = exp(lse_p - lse).  A CTA has some rows of a
+// sequence and eight warps, with 16 dimensions per lane: as many warps share a row, taking its parts in turn, as there are parts.
+constexpr int kJoinWarps = 8;
+__global__ void __launch_bounds__(32 * kJoinWarps) latent_join_kernel(const __grid_constant__ DecodeArgs a, int ctas, int rows_each, int per) {
+    __shared__ float4 sums[kJoinWarps][kValue / 4];
     grid_dep_launch();
     grid_dep_wait();
-    const int per = (a.R + rows_each - 1) / rows_each, b = (int)(blockIdx.x / per), r0 = (int)(blockIdx.x % per) * rows_each;
-    const int me = threadIdx.x & 127, group = threadIdx.x >> 7;
-    const int n = tiles_of(length(a, b));
-    const int64_t before = a.prefix[b], total = a.prefix[a.B];
-    const int64_t share = (total + a.groups - 1) / a.groups;
-    const int64_t first = n > 0 ? before / share : 0, last = n > 0 ? (before + n - 1) / share : 0;
-    if (n > 0 && first == last) return;
+    const int b = (int)blockIdx.x / per, r0 = ((int)blockIdx.x - b * per) * rows_each, end = min(a.R, r0 + rows_each);
+    const int4 span = a.spans[b];
+    const int first = span.x, parts = span.y - span.x + 1;
+    if (parts == 1) return;   // (written by the one CTA that had it, or empty)
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int sharing = rows_each == 1 || parts > 4 ? 8 : (parts > 2 ? 4 : 2), mine = warp % sharing;
     const float* lses = a.parts + (int64_t)ctas * 2 * kRows * kValue;
-    const int parts = (int)min(last - first + 1, (int64_t)kJoinGroups);
-    const int sharing = parts > 4 ? 8 : (parts > 2 ? 4 : (parts > 1 ? 2 : 1)), mine = group % sharing;
-    const int end = min(a.R, r0 + rows_each);
-    for (int base = r0; base < end; base += kJoinGroups / sharing) {   // (all threads come as often to the barriers)
-        const int r = base + group / sharing, rt = r / kRows, row = r % kRows;
-        auto slot = [&](int64_t x) { return ((x * a.row_tiles + rt) * 2 + (x * share >= before ? 0 : 1)) * kRows + row; };   // (a CTA's first stretch is its slot 0)
+    for (int base = r0; base < end; base += kJoinWarps / sharing) {   // (all threads come as often to the barriers)
+        const int r = base + warp / sharing, rt = r / kRows;
+        // a CTA's first stretch is its slot 0
+        auto slot = [&](int p) { return ((int64_t)((first + p) * a.row_tiles + rt) * 2 + (p > 0 || span.z != 0 ? 0 : 1)) * kRows + r % kRows; };
         float ref = -INFINITY, sum = 0.0f;
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (n > 0 && r < end) {
-            for (int64_t x = first + (threadIdx.x & 31); x <= last; x += 32) ref = fmaxf(ref, lses[slot(x)]);
+        float4 acc[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (r < end) {
+            for (int p = lane; p < parts; p += 32) ref = fmaxf(ref, lses[slot(p)]);
 #pragma unroll
             for (int off = 16; off >= 1; off >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, off));
             if (ref == -INFINITY) ref = 0.0f;
-            for (int64_t x = first + (threadIdx.x & 31); x <= last; x += 32) sum += expf(lses[slot(x)] - ref);
+            for (int p = lane; p < parts; p += 32) sum += expf(lses[slot(p)] - ref);
 #pragma unroll
             for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-#pragma unroll 4
-            for (int64_t x = first + mine; x <= last; x += sharing) {
-                const int64_t s = slot(x);
-                const float w = expf(lses[s] - ref);
-                const float4 v = *reinterpret_cast<const float4*>(a.parts + s * kValue + me * 4);
-                acc.x += w * v.x;
-                acc.y += w * v.y;
-                acc.z += w * v.z;
-                acc.w += w * v.w;
+#pragma unroll 2
+            for (int p = mine; p < parts; p += sharing) {
+                const int64_t at = slot(p);
+                const float w = expf(lses[at] - ref);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float4 v = *reinterpret_cast<const float4*>(a.parts + at * kValue + k * 128 + lane * 4);
+                    acc[k].x += w * v.x;
+                    acc[k].y += w * v.y;
+                    acc[k].z += w * v.z;
+                    acc[k].w += w * v.w;
+                }
             }
         }
-        sums[group][me] = acc;
+        if (mine != 0) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sums[warp][k * 32 + lane] = acc[k];
+        }
         __syncthreads();
         if (mine == 0 && r < end) {
-            for (int k = 1; k < sharing; ++k) {
-                const float4 v = sums[group + k][me];
-                acc.x += v.x;
-                acc.y += v.y;
-                acc.z += v.z;
-                acc.w += v.w;
-            }
             const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
-            *reinterpret_cast<uint2*>(a.out + (int64_t)b * a.out_batch + (int64_t)r * a.out_row + me * 4) =
-                make_uint2(pack_bf2(acc.x * inv, acc.y * inv), pack_bf2(acc.z * inv, acc.w * inv));
-            if (me == 0 && a.lse != nullptr) a.lse[(int64_t)b * a.R + r] = sum == 0.0f ? -INFINITY : ref + logf(sum);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                for (int x = 1; x < sharing; ++x) {
+                    const float4 v = sums[warp + x][k * 32 + lane];
+                    acc[k].x += v.x;
+                    acc[k].y += v.y;
+                    acc[k].z += v.z;
+                    acc[k].w += v.w;
+                }
+                *reinterpret_cast<uint2*>(a.out + (int64_t)b * a.out_batch + (int64_t)r * a.out_row + k * 128 + lane * 4) =
+                    make_uint2(pack_bf2(acc[k].x * inv, acc[k].y * inv), pack_bf2(acc[k].z * inv, acc[k].w * inv));
+            }
+            if (lane == 0 && a.lse != nullptr) a.lse[(int64_t)b * a.R + r] = sum == 0.0f ? -INFINITY : ref + logf(sum);
         }
         __syncthreads();
     }
@@ -517,7 +553,7 @@ int groups_for(int64_t row_tiles) {
 
 size_t latent_decode_workspace(const fkda_latent_decode_params& p) {
     const int64_t row_tiles = (p.Tq * p.H + kRows - 1) / kRows;
-    return (size_t)(row_tiles * groups_for(row_tiles)) * 2 * kRows * (kValue + 1) * sizeof(float) + (size_t)(p.B + 1) * sizeof(int64_t);
+    return (size_t)(row_tiles * groups_for(row_tiles)) * 2 * kRows * (kValue + 1) * sizeof(float) + (size_t)p.B * sizeof(int4);
 }
 
 int launch_latent_decode(const fkda_latent_decode_params& p, cudaStream_t stream, int* n_launches) {
@@ -541,7 +577,7 @@ int launch_latent_decode(const fkda_latent_decode_params& p, cudaStream_t stream
     a.box = p.page_size % 64 == 0 ? 64 : (p.page_size % 32 == 0 ? 32 : 16);
     a.max_pages = (int)p.max_pages;
     a.scale = p.scale;
-    a.prefix = reinterpret_cast<int64_t*>(a.parts + (int64_t)a.row_tiles * a.groups * 2 * kRows * (kValue + 1));
+    a.spans = reinterpret_cast<int4*>(a.parts + (int64_t)a.row_tiles * a.groups * 2 * kRows * (kValue + 1));
     DecodeMaps maps;
     const cuuint64_t qdims[3] = {(cuuint64_t)kWidth, (cuuint64_t)a.R, (cuuint64_t)p.B};
     const cuuint64_t qstrides[2] = {(cuuint64_t)p.q_stride[1] * 2, (cuuint64_t)p.q_stride[0] * 2};
@@ -552,13 +588,13 @@ int launch_latent_decode(const fkda_latent_decode_params& p, cudaStream_t stream
     if (!encode_bf16_map(&maps.q, 3, p.q, qdims, qstrides, qbox) || !encode_bf16_map(&maps.cache, 3, p.cache, cdims, cstrides, cbox))
         return FKDA_ERR_LAUNCH;
     const int ctas = a.row_tiles * a.groups;
-    // rows of a joining CTA: one, or more where there are more rows than would be joined at once
-    const int rows_each = (int)std::min<int64_t>(8, std::max<int64_t>(1, p.B * a.R / (2 * device_sm_count())));
-    const int64_t joins = p.B * ((a.R + rows_each - 1) / rows_each);
+    // rows of a joining CTA: one, so that many parts of few rows are joined soon, or eight where there are more rows than the GPU has warps for
+    const int rows_each = p.B * a.R > 4 * device_sm_count() ? 8 : 1, per = (a.R + rows_each - 1) / rows_each;
+    const int64_t joins = p.B * per;
     if (joins > 0x7fffffff) return FKDA_ERR_BAD_SHAPE;
     if (!allow_smem<latent_decode_kernel>(kSmem)) return FKDA_ERR_LAUNCH;
     if (!launch_dependent(latent_decode_kernel, ctas, kThreads, kSmem, stream, a, maps)) return FKDA_ERR_LAUNCH;
-    if (!launch_dependent(latent_join_kernel, joins, 128 * kJoinGroups, 0, stream, a, ctas, rows_each)) return FKDA_ERR_LAUNCH;
+    if (!launch_dependent(latent_join_kernel, joins, 32 * kJoinWarps, 0, stream, a, ctas, rows_each, per)) return FKDA_ERR_LAUNCH;
     *n_launches = 2;
     return FKDA_OK;
 }
