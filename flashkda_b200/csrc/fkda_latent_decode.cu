@@ -337,9 +337,11 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
                         for (int k = 0; k < 4; ++k)
                             if (t * kTok + 8 * i + 2 * tc + (k & 1) >= seen[k >> 1]) s[4 * i + k] = 0xff800000u;
                 }
-                float m[2] = {-INFINITY, -INFINITY};
+                float m[2], most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < 32; ++i) m[(i >> 1) & 1] = fmaxf(m[(i >> 1) & 1], f(s[i]));
+                for (int i = 0; i < 32; i += 2) most[(i >> 1) & 3] = fmaxf(fmaxf(f(s[i]), f(s[i + 1])), most[(i >> 1) & 3]);
+                m[0] = fmaxf(most[0], most[2]);
+                m[1] = fmaxf(most[1], most[3]);
                 bool move[2];
                 float factor[2];
 #pragma unroll
@@ -476,18 +478,19 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
 }
 
 // Joins the parts of the sequences that a cut runs through: sum of w_p O_p over the parts, w_p = exp(lse_p - lse).  A CTA has some rows of a
-// sequence and eight warps, with 16 dimensions per lane: as many warps share a row, taking its parts in turn, as there are parts.
-constexpr int kJoinWarps = 8;
-__global__ void __launch_bounds__(32 * kJoinWarps) latent_join_kernel(const __grid_constant__ DecodeArgs a, int ctas, int rows_each, int per) {
+// sequence, a lane 16 dimensions: as many warps share a row, taking its parts in turn, as there are parts.  One row and 16 warps, so that many
+// parts of few rows are joined soon, or four rows and eight warps, four CTAs per SM, where there are more rows than that.
+template <int kRowsEach, int kJoinWarps>
+__global__ void __launch_bounds__(32 * kJoinWarps, kRowsEach == 1 ? 1 : 4) latent_join_kernel(const __grid_constant__ DecodeArgs a, int ctas, int per) {
     __shared__ float4 sums[kJoinWarps][kValue / 4];
     grid_dep_launch();
     grid_dep_wait();
-    const int b = (int)blockIdx.x / per, r0 = ((int)blockIdx.x - b * per) * rows_each, end = min(a.R, r0 + rows_each);
+    const int b = (int)blockIdx.x / per, r0 = ((int)blockIdx.x - b * per) * kRowsEach, end = min(a.R, r0 + kRowsEach);
     const int4 span = a.spans[b];
     const int first = span.x, parts = span.y - span.x + 1;
     if (parts == 1) return;   // (written by the one CTA that had it, or empty)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int sharing = rows_each == 1 || parts > 4 ? 8 : (parts > 2 ? 4 : 2), mine = warp % sharing;
+    const int sharing = kRowsEach == 1 || parts > 4 ? kJoinWarps : (parts > 2 ? 4 : 2), mine = warp % sharing;
     const float* lses = a.parts + (int64_t)ctas * 2 * kRows * kValue;
     for (int base = r0; base < end; base += kJoinWarps / sharing) {   // (all threads come as often to the barriers)
         const int r = base + warp / sharing, rt = r / kRows;
@@ -498,24 +501,37 @@ __global__ void __launch_bounds__(32 * kJoinWarps) latent_join_kernel(const __gr
 #pragma unroll
         for (int k = 0; k < 4; ++k) acc[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (r < end) {
-            for (int p = lane; p < parts; p += 32) ref = fmaxf(ref, lses[slot(p)]);
+            float4 next[4];   // (on their way while the weights are being made)
+            if (mine < parts) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) next[k] = *reinterpret_cast<const float4*>(a.parts + slot(mine) * kValue + k * 128 + lane * 4);
+            }
+            const float first_lse = lane < parts ? lses[slot(lane)] : -INFINITY;
+            ref = first_lse;
+            for (int p = lane + 32; p < parts; p += 32) ref = fmaxf(ref, lses[slot(p)]);
 #pragma unroll
             for (int off = 16; off >= 1; off >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, off));
             if (ref == -INFINITY) ref = 0.0f;
-            for (int p = lane; p < parts; p += 32) sum += expf(lses[slot(p)] - ref);
+            const float first_weight = expf(first_lse - ref);   // (0 where there is no such part)
+            sum = first_weight;
+            for (int p = lane + 32; p < parts; p += 32) sum += expf(lses[slot(p)] - ref);
 #pragma unroll
             for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-#pragma unroll 2
             for (int p = mine; p < parts; p += sharing) {
-                const int64_t at = slot(p);
-                const float w = expf(lses[at] - ref);
+                float4 v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = next[k];
+                if (p + sharing < parts) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) next[k] = *reinterpret_cast<const float4*>(a.parts + slot(p + sharing) * kValue + k * 128 + lane * 4);
+                }
+                const float w = p < 32 ? __shfl_sync(0xffffffffu, first_weight, p) : expf(lses[slot(p)] - ref);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const float4 v = *reinterpret_cast<const float4*>(a.parts + at * kValue + k * 128 + lane * 4);
-                    acc[k].x += w * v.x;
-                    acc[k].y += w * v.y;
-                    acc[k].z += w * v.z;
-                    acc[k].w += w * v.w;
+                    acc[k].x += w * v[k].x;
+                    acc[k].y += w * v[k].y;
+                    acc[k].z += w * v[k].z;
+                    acc[k].w += w * v[k].w;
                 }
             }
         }
@@ -588,13 +604,14 @@ int launch_latent_decode(const fkda_latent_decode_params& p, cudaStream_t stream
     if (!encode_bf16_map(&maps.q, 3, p.q, qdims, qstrides, qbox) || !encode_bf16_map(&maps.cache, 3, p.cache, cdims, cstrides, cbox))
         return FKDA_ERR_LAUNCH;
     const int ctas = a.row_tiles * a.groups;
-    // rows of a joining CTA: one, so that many parts of few rows are joined soon, or eight where there are more rows than the GPU has warps for
-    const int rows_each = p.B * a.R > 4 * device_sm_count() ? 8 : 1, per = (a.R + rows_each - 1) / rows_each;
+    const int rows_each = p.B * a.R > 4 * device_sm_count() ? 4 : 1, per = (a.R + rows_each - 1) / rows_each;
     const int64_t joins = p.B * per;
     if (joins > 0x7fffffff) return FKDA_ERR_BAD_SHAPE;
     if (!allow_smem<latent_decode_kernel>(kSmem)) return FKDA_ERR_LAUNCH;
     if (!launch_dependent(latent_decode_kernel, ctas, kThreads, kSmem, stream, a, maps)) return FKDA_ERR_LAUNCH;
-    if (!launch_dependent(latent_join_kernel, joins, 32 * kJoinWarps, 0, stream, a, ctas, rows_each, per)) return FKDA_ERR_LAUNCH;
+    if (!(rows_each == 1 ? launch_dependent(latent_join_kernel<1, 16>, joins, 512, 0, stream, a, ctas, per)
+                         : launch_dependent(latent_join_kernel<4, 8>, joins, 256, 0, stream, a, ctas, per)))
+        return FKDA_ERR_LAUNCH;
     *n_launches = 2;
     return FKDA_OK;
 }
