@@ -33,7 +33,8 @@ constexpr int kChunkBytes = 64 * 128;
 constexpr int kStageBytes = kChunks * kChunkBytes;
 constexpr int kStages = 2;                   // (tile g's is g & 1)
 constexpr int kGroups = 5;                   // of a stage, loaded and freed apart: four pairs of 64-dimension tiles, and the rotated one
-constexpr int kThreads = 192;                // softmax warpgroup, a loading and a multiplying warp
+constexpr int kThreads = 256;                // softmax warpgroup, three loading warps (4, 6, 7) and a multiplying one (5)
+constexpr int kLoaders = 3;
 constexpr int kMaxSeqs = kStages * kStageBytes / 4;   // tile counts of all sequences pass through the stages' memory
 constexpr uint32_t kO = 0, kS = 256;         // tensor-memory columns: four output accumulators, two score buffers
 
@@ -167,12 +168,14 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     constexpr uint32_t tmem = 0;   // (all columns are this CTA's)
     Walk walk{(int)uniform(bar.first_seq), (int)uniform(bar.first_tile), as_assumed(smem, bar.tmem) ? (int)uniform(bar.count) : 0, 0, 0, 0};
 
-    if (warp == 4) {
+    if (warp == 4 || warp > 5) {
         // ---- loads: a tile in groups of its dimensions, box by box (pages may end inside it); two tiles on are fetched into L2, so that a
-        //      stage that was freed is full again without waiting for HBM ----
+        //      stage that was freed is full again without waiting for HBM.  A copy takes some 120 cycles to issue, and pages of 16 tokens make
+        //      36 of them per tile: three warps share the groups ----
+        const int who = warp == 4 ? 0 : warp - 5;
         const uint32_t q_addr = smem_u32(q_smem), st_addr = smem_u32(stages), leader = elect_one();
         const int boxes = kTok / a.box;
-        int g = 0, pieces = 0, asked = 0, issued = 0;
+        int g = 0, pieces = 0, asked = 0, issued[2] = {0, 0};   // (tiles of my first and second group)
         bool ok = true;
         auto page_of = [&](int tok) {
             const int page = a.table[(int64_t)walk.b * a.table_stride + tok / a.page];
@@ -186,17 +189,19 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         };
 #pragma unroll 1
         for (; ok && walk.next(a); walk.done(), ++pieces) {
-            fetch_ahead(walk.t + 1);
+            if (who == 2) fetch_ahead(walk.t + 1);
             __syncwarp();
 #pragma unroll 1
             for (int t = walk.t; t < walk.until; ++t, ++g) {
                 const int tok = t * kTok + lane * a.box;
                 const bool load = lane < boxes && tok < walk.len;
                 const int my_page = load ? page_of(tok) : 0, my_row = load ? tok % a.page : 0, n = __popc(__ballot_sync(0xffffffffu, load));
-                fetch_ahead(t + 2);
+                if (who == 2) fetch_ahead(t + 2);
                 __syncwarp();
-#pragma unroll 1
-                for (int j = 0; j < kGroups; ++j) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int j = who + i * kLoaders;
+                    if (j >= kGroups) break;
                     if (g >= kStages) ok = __all_sync(0xffffffffu, wait(&bar.empty[g & 1][j], ((g >> 1) - 1) & 1, &bar.abort));
                     if (!ok) break;
                     const int width = j == kGroups - 1 ? 1 : 2;
@@ -209,10 +214,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
                         load_3d(dst, &maps.cache, j * 128, row, page, full, leader);
                         if (width == 2) load_3d(dst + kChunkBytes, &maps.cache, j * 128 + 64, row, page, full, leader);
                     }
-                    issued = g * kGroups + j + 1;
+                    issued[i] = g + 1;
                 }
                 if (!ok) break;
-                if (t > walk.t) continue;
+                if (t > walk.t || who != 0) continue;
                 // the stretch's queries, once the last one's have been read
                 if (pieces > 0) ok = __all_sync(0xffffffffu, wait(&bar.q_empty, (pieces - 1) & 1, &bar.abort));
                 if (!ok) break;
@@ -225,8 +230,9 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
             if (!ok) break;
         }
         if (asked > 0) drain(&bar.q_full, (asked - 1) & 1);
-#pragma unroll 1
-        for (int k = max(0, issued - kStages * kGroups); k < issued; ++k) drain(&bar.full[k / kGroups % kStages][k % kGroups], (k / kGroups / kStages) & 1);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            for (int k = max(0, issued[i] - kStages); k < issued[i]; ++k) drain(&bar.full[k & 1][who + i * kLoaders], (k >> 1) & 1);
         __syncwarp();
     } else if (warp == 5) {
         // ---- products: two lines of work, each taken up as soon as what it waits for is there: the scores of tile `g`, group by group of its
