@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     fence_proxy_async_smem();   // (the stages are written by copies from here on)
     __syncthreads();
     constexpr uint32_t tmem = 0;   // (all columns are this CTA's)
-    Walk walk{(int)uniform(bar.first_seq), (int)uniform(bar.first_tile), as_assumed(smem, bar.tmem) ? (int)uniform(bar.count) : 0, 0, 0, 0};
+    Walk walk{(int)uniform(bar.first_seq), (int)uniform(bar.first_tile), (int)uniform(as_assumed(smem, bar.tmem) ? bar.count : 0), 0, 0, 0};
 
     if (warp == 4 || warp > 5) {
         // ---- loads: a tile in groups of its dimensions, box by box (pages may end inside it); two tiles on are fetched into L2, so that a

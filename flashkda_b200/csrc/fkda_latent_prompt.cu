@@ -29,7 +29,6 @@ constexpr int kThreads = 384;                // two softmax warpgroups, and one 
 // Registers of a thread: 168 at launch, then 208 for a row's 128 scores and what is made of them; 2 x 208 + 88 = 3 x 168
 constexpr int kRegsRow = 208, kRegsRest = 88;
 static_assert(2 * kRegsRow + kRegsRest <= 3 * 168, "a block has no more");
-constexpr int kSmem = (2 * kKeyTiles + kSlots) * kSlotBytes + 256;
 constexpr uint32_t kS = 0, kO = 256;         // tensor-memory columns: scores (and weights) of the two tiles, outputs
 
 struct PromptMaps {
@@ -41,15 +40,21 @@ struct PromptArgs {
     const int64_t *cu_q, *cu_k;
     int64_t B, T, Tk, N, out_batch, out_token, out_head;
     int H;
+    uint32_t sms;
     float scale;
     int causal;
 };
 
+constexpr int kMaxOrdered = 512;             // packed sequences that are taken in the order of their keys
 struct Bars {
     uint64_t q_full, full[kSlots], empty[kSlots], s_full[2], p_full[2][2], o_done[2], drained;
     uint32_t tmem;
     int abort;
+    int order[kMaxOrdered];
 };
+
+constexpr int kSmem = (2 * kKeyTiles + kSlots) * kSlotBytes + ((int)sizeof(Bars) + 127) / 128 * 128;
+static_assert(kSmem <= 232448, "shared memory of an SM");
 
 // Where a CTA's rows are: sequence, first row, and the extents of queries and keys.
 struct Place {
@@ -57,7 +62,8 @@ struct Place {
     int len_q, len_k, row0;
     bool any;
 };
-__device__ __forceinline__ Place locate(const PromptArgs& a, int64_t slot, int lane) {
+// `order`: the sequences with more keys first, so that a long one does not start when the others are done; or null, as they come.
+__device__ __forceinline__ Place locate(const PromptArgs& a, const int* order, int64_t slot, int lane) {
     Place p;
     if (a.cu_q == nullptr) {
         // long rows first: the last block of every sequence, then the one in front of it, ...
@@ -74,9 +80,9 @@ __device__ __forceinline__ Place locate(const PromptArgs& a, int64_t slot, int l
     p.any = false;
     p.b = 0;
     for (int64_t base = 0; base < a.N; base += 32) {
-        const int64_t n = base + lane;
-        int64_t lo = 0, len = 0;
+        int64_t n = base + lane, lo = 0, len = 0;
         if (n < a.N) {
+            if (order != nullptr) n = order[n];
             lo = a.cu_q[n] < 0 ? 0 : a.cu_q[n];
             const int64_t hi = a.cu_q[n + 1] > a.T ? a.T : a.cu_q[n + 1];
             len = hi > lo ? hi - lo : 0;
@@ -92,7 +98,7 @@ __device__ __forceinline__ Place locate(const PromptArgs& a, int64_t slot, int l
         if (behind != 0) {
             const int src = __ffs(behind) - 1;
             const int64_t first = seen + __shfl_sync(0xffffffffu, upto - tiles, src);
-            const int64_t seq = base + src;
+            const int64_t seq = __shfl_sync(0xffffffffu, n, src);
             p.q0 = __shfl_sync(0xffffffffu, lo, src);
             p.len_q = (int)__shfl_sync(0xffffffffu, len, src);
             p.row0 = (int)((p.len_q + kRows - 1) / kRows - 1 - (slot - first)) * kRows;
@@ -105,6 +111,23 @@ __device__ __forceinline__ Place locate(const PromptArgs& a, int64_t slot, int l
         seen += __shfl_sync(0xffffffffu, upto, 31);
     }
     return p;
+}
+
+// (Not inlined: with its loops in sight the compiler no longer sees the warps as converged, and the descriptors of the products leave the
+// uniform registers: 546 -> 960 us for 8 192 tokens of 32 heads.)
+__device__ __noinline__ void make_order(const PromptArgs& a, int* lens, int* order) {
+    for (int i = threadIdx.x; i < a.N; i += kThreads) lens[i] = (int)(a.cu_k[i + 1] - a.cu_k[i]);
+    fence_proxy_async_smem();
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.N; i += kThreads) {
+        const int len = lens[i];
+        int rank = 0;
+#pragma unroll 1
+        for (int j = 0; j < (int)a.N; ++j) rank += lens[j] > len || (lens[j] == len && j < i) ? 1 : 0;
+        order[rank] = i;
+    }
+    fence_proxy_async_smem();
+    __syncthreads();
 }
 
 __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ PromptMaps maps) {
@@ -128,7 +151,12 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
     __syncthreads();
     fence_after();
     constexpr uint32_t tmem = 0;   // (all columns are this CTA's)
-    Place p = locate(a, blockIdx.x / a.H, lane);
+    const int* order = nullptr;
+    if (a.cu_q != nullptr && a.N > 1 && a.N <= kMaxOrdered && gridDim.x > a.sms) {
+        make_order(a, reinterpret_cast<int*>(ring), bar.order);
+        order = bar.order;
+    }
+    Place p = locate(a, order, blockIdx.x / a.H, lane);
     p.any = p.any && as_assumed(smem, bar.tmem);
     const int h = (int)(blockIdx.x % (uint32_t)a.H);
     // key blocks of the two tiles: a row sees the keys up to its own place counted from the ends
@@ -385,6 +413,7 @@ int launch_latent_prompt(const fkda_latent_params& p, cudaStream_t stream, int* 
     a.H = (int)p.H;
     a.scale = p.scale;
     a.causal = p.causal;
+    a.sms = (uint32_t)device_sm_count();
     const int64_t tiles = (p.T + kRows - 1) / kRows;
     const int64_t ctas = (p.cu_seqlens != nullptr ? p.T / kRows + p.N : tiles * p.B) * p.H;   // (ragged: never fewer than there are)
     if (ctas > 0x7fffffff) return FKDA_ERR_BAD_SHAPE;

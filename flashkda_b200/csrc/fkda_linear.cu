@@ -46,6 +46,10 @@ struct LinearArgs {
     int H, group;      // value heads, value heads of a key head
     float scale;
     bool state_fp32, skip_single;
+    bool ordered;           // packed sequences: the longest first
+    int seg_len, seg_rows;  // tokens of a segment, 0: every chain is walked in one piece; rows that the workspace has
+    float* seg_state;       // [segment][head][128][128], and behind them
+    float* seg_decay;       // [segment][head]
 };
 struct LinearMaps {
     CUtensorMap q, k, v, out;
@@ -60,7 +64,7 @@ struct Bars {
     uint64_t full[kStages], empty[kStages], dec_full[kStages], dec_empty[kStages], score, score_free, p_full[2], p_free[2], out_full, out_free, scaled[2], s_done[2], copy_free,
         w_full[2], drained[2];
     uint32_t tmem;
-    int abort;
+    int abort, chosen;
 };
 constexpr int kSmem = kOffBars + ((int)sizeof(Bars) + 127) / 128 * 128;
 static_assert(kSmem <= 232448, "shared memory of an SM");
@@ -69,41 +73,72 @@ constexpr float kLog2e = 1.4426950408889634f;
 // exp(-100) is nothing in fp32; a decay below it (minus infinity to start afresh) would make differences of sums meaningless.
 __device__ __forceinline__ float log2_decay(float g) { return (g < -100.0f ? -100.0f : g) * kLog2e; }
 
+// What a CTA walks: a sequence's head, or one segment of it.
 struct Chain {
-    int64_t n, b, t0;
+    int64_t n, b, t0;      // sequence, batch row, first token
     int h, len;
+    int seg, segs;         // segment of the sequence's, of which there are `segs`
+    int64_t slot;          // of the segment and head in the workspace
 };
-__device__ __forceinline__ Chain locate(const LinearArgs& a, int64_t chain) {
+__device__ __forceinline__ int seq_len(const LinearArgs& a, int64_t n, int64_t* first) {
+    const int64_t lo = a.cu[n] < 0 ? 0 : a.cu[n], hi = a.cu[n + 1] > a.T ? a.T : a.cu[n + 1];
+    *first = lo;
+    return hi > lo ? (int)(hi - lo) : 0;
+}
+__device__ __forceinline__ int segments(const LinearArgs& a, int len) { return a.seg_len == 0 || len == 0 ? 1 : (len + a.seg_len - 1) / a.seg_len; }
+// `row`: of (sequence, segment) pairs in order; len < 0: there are fewer.
+__device__ __forceinline__ Chain locate(const LinearArgs& a, int64_t row, int h) {
     Chain c;
-    c.n = chain / a.H;
-    c.h = (int)(chain - c.n * a.H);
+    c.h = h;
+    c.slot = row * a.H + h;
+    c.b = 0;
+    c.seg = 0;
+    c.segs = 1;
     if (a.cu == nullptr) {
+        c.segs = segments(a, (int)a.T);
+        c.n = c.segs == 1 ? row : row / c.segs;
+        c.seg = (int)(row - c.n * c.segs);
         c.b = c.n;
         c.t0 = 0;
-        c.len = (int)a.T;
-    } else {
-        c.b = 0;
-        const int64_t lo = a.cu[c.n] < 0 ? 0 : a.cu[c.n], hi = a.cu[c.n + 1] > a.T ? a.T : a.cu[c.n + 1];
-        c.t0 = lo;
-        c.len = hi > lo ? (int)(hi - lo) : 0;
+        c.len = c.n < a.N ? (int)a.T : -1;
+    } else if (a.seg_len == 0) {
+        c.n = row;
+        c.len = row < a.N ? seq_len(a, row, &c.t0) : -1;
+    } else {   // (few sequences)
+        int64_t seen = 0;
+        c.len = -1;
+        for (c.n = 0; c.n < a.N; ++c.n) {
+            const int len = seq_len(a, c.n, &c.t0);
+            c.segs = segments(a, len);
+            if (row < seen + c.segs) {
+                c.seg = (int)(row - seen);
+                if (seen + c.segs <= a.seg_rows) c.len = len;   // (always, unless cu_seqlens runs backwards)
+                break;
+            }
+            seen += c.segs;
+        }
+    }
+    if (c.len > 0 && c.segs > 1) {
+        c.t0 += (int64_t)c.seg * a.seg_len;
+        c.len = min(a.seg_len, c.len - c.seg * a.seg_len);
     }
     return c;
 }
 
-// 32 numbers of a row of the state
-__device__ __forceinline__ void load_state32(const LinearArgs& a, int64_t at, uint32_t* r) {
-    if (a.h0 == nullptr) {
+// 32 numbers of a row of a state
+__device__ __forceinline__ void load_state32(const void* from, bool fp32, int64_t at, uint32_t* r) {
+    if (from == nullptr) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) r[i] = 0u;
-    } else if (a.state_fp32) {
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(a.h0) + at);
+    } else if (fp32) {
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(from) + at);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const uint4 x = src[i];
             r[4 * i] = x.x; r[4 * i + 1] = x.y; r[4 * i + 2] = x.z; r[4 * i + 3] = x.w;
         }
     } else {
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.h0) + at);
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(from) + at);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint4 x = src[i];
@@ -116,13 +151,13 @@ __device__ __forceinline__ void load_state32(const LinearArgs& a, int64_t at, ui
         }
     }
 }
-__device__ __forceinline__ void store_state32(const LinearArgs& a, int64_t at, const uint32_t* r) {
-    if (a.state_fp32) {
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<float*>(a.hT) + at);
+__device__ __forceinline__ void store_state32(void* to, bool fp32, int64_t at, const uint32_t* r) {
+    if (fp32) {
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<float*>(to) + at);
 #pragma unroll
         for (int i = 0; i < 8; ++i) dst[i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
     } else {
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.hT) + at);
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(to) + at);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             dst[i] = make_uint4(pack_bf2(f(r[8 * i]), f(r[8 * i + 1])), pack_bf2(f(r[8 * i + 2]), f(r[8 * i + 3])),
@@ -130,12 +165,15 @@ __device__ __forceinline__ void store_state32(const LinearArgs& a, int64_t at, c
     }
 }
 
+// kStates: only the state that each segment but the last leaves behind a zero one (the first: behind the initial state), and the
+// product of its decays.
+template <bool kStates>
 __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_constant__ LinearArgs a, const __grid_constant__ LinearMaps maps) {
     extern __shared__ __align__(1024) uint8_t smem[];
     Bars& bar = *reinterpret_cast<Bars*>(smem + kOffBars);
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kStages; ++i) mbar_init(&bar.full[i], 1), mbar_init(&bar.empty[i], 2), mbar_init(&bar.dec_full[i], 1), mbar_init(&bar.dec_empty[i], 24);
+        for (int i = 0; i < kStages; ++i) mbar_init(&bar.full[i], 1), mbar_init(&bar.empty[i], kStates ? 1 : 2), mbar_init(&bar.dec_full[i], 1), mbar_init(&bar.dec_empty[i], kStates ? 12 : 24);
         for (int i = 0; i < 2; ++i) mbar_init(&bar.p_full[i], 128), mbar_init(&bar.p_free[i], 1), mbar_init(&bar.w_full[i], 128);
         mbar_init(&bar.score, 1);
         mbar_init(&bar.score_free, 128);
@@ -154,8 +192,26 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     __syncthreads();
     fence_after();
     constexpr uint32_t tmem = 0;   // (all columns are this CTA's)
-    const Chain ch = locate(a, blockIdx.x);
-    const bool mine = !(a.skip_single && ch.len <= 1) && as_assumed(smem, bar.tmem);
+    int row = (int)(blockIdx.x / (uint32_t)a.H);
+    if (a.ordered) {   // the sequence that as many others come before as rows are in front of mine
+        int* lens = reinterpret_cast<int*>(smem);
+        int64_t first;
+        const int me = threadIdx.x, len = me < a.N ? seq_len(a, me, &first) : 0;
+        if (me < a.N) lens[me] = len;
+        fence_proxy_async_smem();
+        __syncthreads();
+        int rank = 0;
+        if (me < a.N)
+#pragma unroll 4
+            for (int i = 0; i < (int)a.N; ++i) rank += lens[i] > len || (lens[i] == len && i < me) ? 1 : 0;
+        if (me < a.N && rank == row) bar.chosen = me;
+        fence_proxy_async_smem();
+        __syncthreads();
+        row = bar.chosen;
+    }
+    const Chain ch = locate(a, row, (int)(blockIdx.x % (uint32_t)a.H));
+    const bool last = ch.seg + 1 == ch.segs;
+    const bool mine = ch.len >= 0 && !(a.skip_single && ch.len <= 1) && !(kStates && last) && as_assumed(smem, bar.tmem);
     const int n = uniform(mine ? (ch.len + kC - 1) / kC : 0);
 
     if (warp == 24) {
@@ -167,10 +223,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         for (; c < n; ++c) {
             if (c >= kStages && !__all_sync(0xffffffffu, wait(&bar.empty[stage], phase, &bar.abort))) break;
             const uint32_t dst = base + stage * kStageBytes;
-            expect(&bar.full[stage], kStageBytes, leader);
+            expect(&bar.full[stage], kStates ? 2 * kOperandBytes : kStageBytes, leader);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                load_4d(dst + x * kTileBytes, &maps.q, x * 64, key_head, t0 + c * kC, row, &bar.full[stage], leader);
+                if (!kStates) load_4d(dst + x * kTileBytes, &maps.q, x * 64, key_head, t0 + c * kC, row, &bar.full[stage], leader);
                 load_4d(dst + kOperandBytes + x * kTileBytes, &maps.k, x * 64, key_head, t0 + c * kC, row, &bar.full[stage], leader);
                 load_4d(dst + 2 * kOperandBytes + x * kTileBytes, &maps.v, x * 64, head, t0 + c * kC, row, &bar.full[stage], leader);
             }
@@ -206,16 +262,18 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
                 }
                 if (c + 1 < n) {
                     wait_warp(&bar.full[stage], phase, &bar.abort);
+                    k = desc(base + stage * kStageBytes + kOperandBytes);
+                    if (!kStates) {
                     if (c >= 0) wait_warp(&bar.score_free, c & 1, &bar.abort);
                     fence_after();
                     const uint32_t q = desc(base + stage * kStageBytes);
-                    k = desc(base + stage * kStageBytes + kOperandBytes);
 #pragma unroll 1
                     for (int x = 0; x < 2; ++x)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             mma_ss(tmem + kScore, q + x * (kTileBytes / 16) + i * 2, k + x * (kTileBytes / 16) + i * 2, kIdScore, (x | i) != 0, leader);
                     commit(&bar.score, leader);
+                    }
                     if (++stage == kStages) stage = 0, phase ^= 1;
                 }
             }
@@ -224,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         }
     } else if (warp == 27) {
         // ---- products of the outputs ----
-        if (n > 0) {
+        if (n > 0 && !kStates) {
             const uint32_t base = smem_u32(smem), leader = elect_one();
             constexpr uint32_t kIdO1 = idesc(128, 64, false, false), kIdO2 = idesc(128, 64, true, false);
             int stage = 0, phase = 0;
@@ -257,6 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         }
     } else if (warp == 26) {
         // ---- decays: lane l has tokens 2 l and 2 l + 1 of a chunk ----
+        float all = 0.0f;
         const float* g = a.g + ch.b * a.g_batch + ch.t0 * a.g_token + ch.h * a.g_head;
 #pragma unroll 1
         for (int c = 0; c < n; ++c) {
@@ -277,19 +336,32 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
             *reinterpret_cast<float2*>(&d.eG[2 * lane]) = make_float2(ex2_approx(G0) * a.scale, ex2_approx(G1) * a.scale);
             *reinterpret_cast<float2*>(&d.w[2 * lane]) = make_float2(ex2_approx(w0), ex2_approx(w1));
             if (lane == 0) d.total = ex2_approx(from);
+            all += from;
             __syncwarp();
             if (lane == 0) arrive(&bar.dec_full[c % kStages]);
         }
+        if (kStates && n > 0 && lane == 0) a.seg_decay[ch.slot] = ex2_approx(all);
     } else if (warp < 4) {
         // ---- state: thread = row (dimension of v); decayed in place, with a bf16 copy of what it was for the product with q ----
         const int v = warp * 32 + lane;
         const uint32_t lanes = (uint32_t)(warp * 32) << 16, ts = tmem + kS + lanes;
-        const int64_t at = ((ch.n * a.H + ch.h) * kD + v) * (int64_t)kD;
+        const int64_t at = ((ch.n * a.H + ch.h) * kD + v) * (int64_t)kD, seg_at = (ch.slot * kD + v) * (int64_t)kD;
+        // the state in front: the call's, a copy of it (its buffer may be the final state's, which the last segment writes while the first
+        // one starts), or what the segment in front leaves
+        const void* from = a.h0;
+        bool fp32 = a.state_fp32;
+        int64_t from_at = at;
+        if (kStates && ch.seg > 0 && !last) from = nullptr;
+        if (!kStates && ch.segs > 1 && (ch.seg > 0 || a.h0 != nullptr)) {
+            from = a.seg_state;
+            fp32 = true;
+            from_at = seg_at + (int64_t)(ch.seg > 0 ? -1 : ch.segs - 1) * a.H * (kD * kD);
+        }
         if (n > 0) {
 #pragma unroll 1
             for (int x = 0; x < 4; ++x) {
                 uint32_t r[32];
-                load_state32(a, at + x * 32, r);
+                load_state32(from, fp32, from_at + x * 32, r);
                 st32(ts + x * 32, r);
             }
             wait_st();
@@ -301,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
             const float total = bar.decay[s].total;
             __syncwarp();
             mbar_arrive_lane0(&bar.dec_empty[s], lane);
-            if (c > 0) wait_warp(&bar.copy_free, (c - 1) & 1, &bar.abort);
+            if (!kStates && c > 0) wait_warp(&bar.copy_free, (c - 1) & 1, &bar.abort);
 #pragma unroll 1
             for (int h = 0; h < 2; ++h) {
                 if (c > 0) {
@@ -319,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
                         mul2(r[2 * i], r[2 * i + 1], total, total);
                     }
                     st32(ts + x * 32, r);
-                    st16(tmem + kCopy + lanes + x * 16, copy);
+                    if (!kStates) st16(tmem + kCopy + lanes + x * 16, copy);
                 }
                 wait_st();
                 fence_before();
@@ -331,22 +403,25 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
             wait_warp(&bar.s_done[1], (n - 1) & 1, &bar.abort);
             fence_after();
         }
-        if (mine && a.hT != nullptr) {
+        const bool keeps = kStates ? ch.len >= 0 && ch.segs > 1 && (!last || a.h0 != nullptr) : mine && last && a.hT != nullptr;
+        if (keeps) {
 #pragma unroll 1
             for (int x = 0; x < 4; ++x) {
                 uint32_t r[32];
                 if (n > 0) {
                     ld32(ts + x * 32, r);
                     wait_ld();
-                } else {
-                    load_state32(a, at + x * 32, r);
+                } else {   // (an empty sequence, or the copy of the initial state in the last segment's place)
+                    load_state32(from, fp32, from_at + x * 32, r);
                 }
-                store_state32(a, at + x * 32, r);
+                if (kStates) store_state32(a.seg_state, true, seg_at + x * 32, r);
+                else store_state32(a.hT, a.state_fp32, at + x * 32, r);
             }
         }
         fence_before();
     } else if (warp < 8) {
         // ---- scores to weights: warp w has rows (queries) 16 w .. 16 w + 15, thread 4 g + t rows g and g + 8 of these ----
+        if (!kStates) {
         const int w = warp - 4, gr = lane >> 2, tc = lane & 3;
         const int r0 = w * 16 + gr, r1 = r0 + 8;
 #pragma unroll 1
@@ -388,9 +463,11 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
             __syncwarp();
             mbar_arrive_lane0(&bar.dec_empty[c % kStages], lane);
         }
+        }
     } else if (warp < 16) {
         // ---- outputs: fragments of 16 dimensions of v x 32 tokens, stored transposed as rows of tokens, which one copy takes away (or the
         //      warps themselves, where the chunk's last rows are not the sequence's) ----
+        if (!kStates) {
         const int w = warp & 3, half = (warp - 8) >> 2, tc = lane & 3, me = threadIdx.x & 255;   // a warpgroup has 32 of the tokens
         // the lane's row address within four 8 x 8 blocks (two of tokens x two of dimensions)
         const int token = (lane & 7) + ((lane >> 4) << 3), unit = (w & 1) * 4 + ((lane >> 3) & 1);
@@ -448,6 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
             }
         }
         if (me == 0) bulk_wait_group<0>();
+        }
     } else {
         // ---- weighted values: transposed reads give thread 4 g + t of warp w the token pairs 8 b + 2 t, + 1 of dimensions g, g + 8, g + 16
         //      and g + 24 of the warp's 32, as the A operand wants them; what is behind the sequence's end becomes nothing ----
@@ -524,11 +602,16 @@ __global__ void __launch_bounds__(128) linear_step_kernel(const __grid_constant_
     grid_dep_launch();
     grid_dep_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t chain = blockIdx.x / kStepSplit;
-    const Chain ch = locate(a, chain);
+    const uint32_t chain = blockIdx.x / kStepSplit;
+    Chain ch;
+    ch.n = chain / (uint32_t)a.H;
+    ch.h = (int)(chain % (uint32_t)a.H);
+    ch.b = a.cu == nullptr ? ch.n : 0;
+    ch.t0 = 0;
+    ch.len = a.cu == nullptr ? (int)a.T : seq_len(a, ch.n, &ch.t0);
     if (ch.len > 1) return;   // (the chunk kernel's)
     const int row0 = (warp * kStepSplit + (int)(blockIdx.x % kStepSplit)) * kStepRows;
-    const int64_t at = (chain * kD + row0) * (int64_t)kD + lane * 4;
+    const int64_t at = ((int64_t)chain * kD + row0) * kD + lane * 4;
     float s[kStepRows][4];
     if (a.h0 == nullptr) {
 #pragma unroll
@@ -589,9 +672,67 @@ __global__ void __launch_bounds__(128) linear_step_kernel(const __grid_constant_
     }
 }
 
+// The states in front of the segments: what a segment left behind a zero state, plus what came in, decayed by it.  A CTA: a sixteenth
+// of a chain's states, a float4 per thread.
+__global__ void __launch_bounds__(256) linear_carry_kernel(const __grid_constant__ LinearArgs a) {
+    grid_dep_launch();
+    grid_dep_wait();
+    const int64_t chain = blockIdx.x / 16, n = chain / a.H;
+    int64_t row = 0, first;
+    int segs = segments(a, (int)a.T);
+    if (a.cu == nullptr) {
+        row = n * segs;
+    } else {
+        for (int64_t i = 0; i < n; ++i) row += segments(a, seq_len(a, i, &first));
+        segs = segments(a, seq_len(a, n, &first));
+    }
+    if (row + segs > a.seg_rows) return;
+    const int64_t slot = row * a.H + chain % a.H;
+    float4* at = reinterpret_cast<float4*>(a.seg_state) + slot * (kD * kD / 4) + (blockIdx.x % 16) * 256 + threadIdx.x;
+    const int64_t step = (int64_t)a.H * (kD * kD / 4);
+    float4 x = *at;
+#pragma unroll 4
+    for (int s = 1; s + 1 < segs; ++s) {
+        const float decay = a.seg_decay[slot + (int64_t)s * a.H];
+        float4 y = at[s * step];
+        y.x = __fmaf_rn(decay, x.x, y.x);
+        y.y = __fmaf_rn(decay, x.y, y.y);
+        y.z = __fmaf_rn(decay, x.z, y.z);
+        y.w = __fmaf_rn(decay, x.w, y.w);
+        at[s * step] = y;
+        x = y;
+    }
+}
+
+// Tokens of a segment, 0 for none, and how many (sequence, segment) rows there are at most.  Segments put the idle SMs of few long
+// chains to work, for half of a chunk's work more: the states are made first, without outputs.
+struct Segments {
+    int len;
+    int64_t rows;
+};
+Segments plan(const fkda_linear_params& p) {
+    const Segments none{0, p.N};
+    const int sms = device_sm_count();
+    const bool packed = p.cu_seqlens != nullptr;
+    const int64_t rows = sms / p.H - (packed ? p.N : 0);   // (every packed sequence has one that is not full)
+    const int64_t pieces = packed ? rows : rows / p.N, tokens = p.T;
+    if (pieces < 2 || p.N > 64) return none;
+    const int64_t len = ((tokens + pieces - 1) / pieces + kC - 1) / kC * kC;
+    const int64_t segs = (tokens + len - 1) / len;
+    if (segs < 2) return none;
+    // in units of a chunk of the whole walk: one with states only takes about 0.7, the two more launches and starts 8.  (Of a packed batch
+    // only the tokens are known: its longest sequence is taken to have 2 / (N + 1) of them.)
+    const double whole = (double)tokens / kC * (packed ? 2.0 / (double)(p.N + 1) : 1.0), split = (double)len / kC * 1.7 + 8;
+    if (split > whole) return none;
+    return Segments{(int)len, packed ? tokens / len + p.N : segs * p.N};
+}
+
 }  // namespace
 
-size_t linear_workspace(const fkda_linear_params&) { return 0; }
+size_t linear_workspace(const fkda_linear_params& p) {
+    const Segments seg = plan(p);
+    return seg.len == 0 ? 0 : (size_t)(seg.rows * p.H) * (kD * kD + 1) * sizeof(float);
+}
 
 int launch_linear(const fkda_linear_params& p, cudaStream_t stream, int* n_launches) {
     LinearArgs a;
@@ -620,6 +761,9 @@ int launch_linear(const fkda_linear_params& p, cudaStream_t stream, int* n_launc
     const bool single = p.cu_seqlens == nullptr ? p.T <= 1 : p.T < 2 * p.N;
     const bool chunks = p.cu_seqlens == nullptr ? p.T > 1 : p.T > 1;
     a.skip_single = single;
+    a.ordered = false;
+    a.seg_len = a.seg_rows = 0;
+    a.seg_state = a.seg_decay = nullptr;
     int launches = 0;
     if (single) {
         if (!launch_dependent(linear_step_kernel, chains * kStepSplit, 128, 0, stream, a)) return FKDA_ERR_LAUNCH;
@@ -636,8 +780,22 @@ int launch_linear(const fkda_linear_params& p, cudaStream_t stream, int* n_launc
         if (!map4(&maps.q, p.q, p.Hk, p.q_stride) || !map4(&maps.k, p.k, p.Hk, p.k_stride) || !map4(&maps.v, p.v, p.H, p.v_stride) ||
             !map4(&maps.out, p.out, p.H, p.out_stride))
             return FKDA_ERR_LAUNCH;
-        if (!allow_smem<linear_chunk_kernel>(kSmem)) return FKDA_ERR_LAUNCH;
-        if (!launch_dependent(linear_chunk_kernel, chains, kThreads, kSmem, stream, a, maps)) return FKDA_ERR_LAUNCH;
+        const Segments seg = single ? Segments{0, p.N} : plan(p);
+        a.seg_len = seg.len;
+        a.seg_rows = (int)seg.rows;
+        a.seg_state = static_cast<float*>(p.workspace);
+        a.seg_decay = a.seg_state + seg.rows * p.H * (kD * kD);
+        // the longest first where not all run at once
+        a.ordered = p.cu_seqlens != nullptr && seg.len == 0 && p.N > 1 && p.N <= kThreads && chains > device_sm_count();
+        if (!allow_smem<linear_chunk_kernel<false>>(kSmem)) return FKDA_ERR_LAUNCH;
+        if (seg.len > 0) {
+            if (!allow_smem<linear_chunk_kernel<true>>(kSmem)) return FKDA_ERR_LAUNCH;
+            if (!launch_dependent(linear_chunk_kernel<true>, seg.rows * p.H, kThreads, kSmem, stream, a, maps) ||
+                !launch_dependent(linear_carry_kernel, chains * 16, 256, 0, stream, a))
+                return FKDA_ERR_LAUNCH;
+            launches += 2;
+        }
+        if (!launch_dependent(linear_chunk_kernel<false>, seg.rows * p.H, kThreads, kSmem, stream, a, maps)) return FKDA_ERR_LAUNCH;
         ++launches;
     }
     *n_launches = launches;

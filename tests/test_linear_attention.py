@@ -143,6 +143,54 @@ def test_state_in_place_and_continued(T):
     check_linear(d, [2 * T], SCALE, d["out"], hT)
 
 
+SEGMENTED = [([770], "fp32"), ([705], "none"), ([1000, 1000], "bf16"), ([700, 1, 90, 0, 1450], "fp32"), ([2, 2300, 64], "none")]
+
+
+@gpu
+@pytest.mark.parametrize("lens,state", SEGMENTED, ids=str)
+@pytest.mark.parametrize("in_place", [False, True])
+def test_few_long_chains_in_segments(lens, state, in_place):
+    packed = len(set(lens)) > 1
+    d = linear_inputs(lens, 2, 1, seed=14, packed=packed, strong=0.1)
+    d["h0"] = d["h0"].to(torch.bfloat16 if state == "bf16" else torch.float32)
+    T = sum(lens) if packed else lens[0]
+    size = flashkda_b200.linear_attention_workspace_size(1 if packed else len(lens), T, 2, len(lens), packed)
+    assert size > 0
+    state0 = d["h0"].clone() if state != "none" else None
+    hT = state0 if in_place and state0 is not None else torch.full_like(d["h0"], 9.0)
+    call(d, h0=state0, hT=hT, workspace=torch.full((size,), 255, dtype=torch.uint8, device="cuda"))
+    assert flashkda_b200.last_launch_count() == 3
+    check_linear(d, lens, SCALE, d["out"], hT, state != "none")
+    # without a final state, and in scratch of the call's own
+    want = d["out"].clone()
+    d["out"].zero_()
+    call(d, h0=d["h0"] if state != "none" else None)
+    assert torch.equal(d["out"], want)
+
+
+@gpu
+def test_segments_captured_and_replayed_with_other_lengths():
+    lens = [700, 1, 90, 0, 1450]
+    d = linear_inputs(lens, 2, seed=15, packed=True)
+    ws = torch.empty(flashkda_b200.linear_attention_workspace_size(1, sum(lens), 2, 5, True), dtype=torch.uint8, device="cuda")
+    hT = torch.zeros(5, 2, 128, 128, device="cuda")
+    call(d, h0=d["h0"], hT=hT, workspace=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(d, h0=d["h0"], hT=hT, workspace=ws)
+    other = [3, 1200, 64, 300, 674]
+    d["cu"].copy_(torch.tensor([0] + other).cumsum(0))
+    d["out"].fill_(7.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    check_linear(d, other, SCALE, d["out"], hT)
+    with pytest.raises(RuntimeError, match="workspace must be"):
+        call(d, h0=d["h0"], hT=hT, workspace=ws[:-1])
+    with pytest.raises(RuntimeError, match="workspace missing, misaligned"):
+        call(d, h0=d["h0"], hT=hT, workspace=torch.empty(ws.numel() + 64, dtype=torch.uint8, device="cuda")[16:])
+
+
 @gpu
 def test_nothing_of_a_neighbour_or_of_padding_is_used():
     """A sequence between two that hold NaN and infinities."""
