@@ -75,7 +75,9 @@ __device__ __forceinline__ int length(const DecodeArgs& a, int b) {
 struct Walk {
     int b, t, left;
     int len, tiles, until;   // of the current stretch: [t, until)
-    __device__ __forceinline__ bool next(const DecodeArgs& a) {
+    // (Not inlined: with its loop in sight the compiler no longer sees the warps as converged, and the descriptors of the products leave
+    // the uniform registers.)
+    __device__ __noinline__ bool next(const DecodeArgs& a) {
         if (left <= 0) return false;
         len = length(a, b);
         tiles = tiles_of(len);

@@ -86,8 +86,10 @@ __device__ __forceinline__ int seq_len(const LinearArgs& a, int64_t n, int64_t* 
     return hi > lo ? (int)(hi - lo) : 0;
 }
 __device__ __forceinline__ int segments(const LinearArgs& a, int len) { return a.seg_len == 0 || len == 0 ? 1 : (len + a.seg_len - 1) / a.seg_len; }
+// (Not inlined, nor is the next one: with their loops in sight the compiler no longer sees the warps as converged, and the descriptors
+// of the products leave the uniform registers.)
 // `row`: of (sequence, segment) pairs in order; len < 0: there are fewer.
-__device__ __forceinline__ Chain locate(const LinearArgs& a, int64_t row, int h) {
+__device__ __noinline__ Chain locate(const LinearArgs& a, int64_t row, int h) {
     Chain c;
     c.h = h;
     c.slot = row * a.H + h;
@@ -123,6 +125,22 @@ __device__ __forceinline__ Chain locate(const LinearArgs& a, int64_t row, int h)
         c.len = min(a.seg_len, c.len - c.seg * a.seg_len);
     }
     return c;
+}
+
+// The sequence that `row` others come before: by length, then by number.
+__device__ __noinline__ void in_order(const LinearArgs& a, int row, int* lens, int* chosen) {
+    int64_t first;
+    const int me = threadIdx.x, len = me < a.N ? seq_len(a, me, &first) : 0;
+    if (me < a.N) lens[me] = len;
+    fence_proxy_async_smem();
+    __syncthreads();
+    int rank = 0;
+    if (me < a.N)
+#pragma unroll 1
+        for (int i = 0; i < (int)a.N; ++i) rank += lens[i] > len || (lens[i] == len && i < me) ? 1 : 0;
+    if (me < a.N && rank == row) *chosen = me;
+    fence_proxy_async_smem();
+    __syncthreads();
 }
 
 // 32 numbers of a row of a state
@@ -194,19 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     constexpr uint32_t tmem = 0;   // (all columns are this CTA's)
     int row = (int)(blockIdx.x / (uint32_t)a.H);
     if (a.ordered) {   // the sequence that as many others come before as rows are in front of mine
-        int* lens = reinterpret_cast<int*>(smem);
-        int64_t first;
-        const int me = threadIdx.x, len = me < a.N ? seq_len(a, me, &first) : 0;
-        if (me < a.N) lens[me] = len;
-        fence_proxy_async_smem();
-        __syncthreads();
-        int rank = 0;
-        if (me < a.N)
-#pragma unroll 4
-            for (int i = 0; i < (int)a.N; ++i) rank += lens[i] > len || (lens[i] == len && i < me) ? 1 : 0;
-        if (me < a.N && rank == row) bar.chosen = me;
-        fence_proxy_async_smem();
-        __syncthreads();
+        in_order(a, row, reinterpret_cast<int*>(smem), &bar.chosen);
         row = bar.chosen;
     }
     const Chain ch = locate(a, row, (int)(blockIdx.x % (uint32_t)a.H));
