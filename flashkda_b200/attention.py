@@ -80,7 +80,7 @@ def latent_attention_decode(q, cache, block_table, cache_lens, scale, out, lse=N
     tokens in the cache, the new ones among them; out: bf16 ``[B, Tq, H, 512]``; lse: fp32 ``[B, Tq, H]``.  New token ``i`` sees the
     first ``len - Tq + 1 + i`` tokens; one that sees none gets 0 and ``lse`` minus infinity.  In q and out the new tokens lie ``H``
     heads apart.  What a page holds behind a sequence's last token is not used; entries of ``block_table`` that are no page number
-    read page 0.  ``scale`` must be positive.  ``workspace``: optional caller-owned uint8 scratch
+    read page 0.  At most 36 864 sequences; ``scale`` must be positive.  ``workspace``: optional caller-owned uint8 scratch
     (``latent_decode_workspace_size``).
     """
     _latent_attention_decode(q, cache, block_table, cache_lens, scale, out, lse, workspace)

@@ -606,11 +606,12 @@ int launch_latent_decode(const fkda_latent_decode_params& p, cudaStream_t stream
     const cuuint64_t qdims[3] = {(cuuint64_t)kWidth, (cuuint64_t)a.R, (cuuint64_t)p.B};
     const cuuint64_t qstrides[2] = {(cuuint64_t)p.q_stride[1] * 2, (cuuint64_t)p.q_stride[0] * 2};
     const cuuint32_t qbox[3] = {64u, (cuuint32_t)kRows, 1u};
-    const cuuint64_t cdims[3] = {(cuuint64_t)kWidth, (cuuint64_t)p.page_size, (cuuint64_t)(p.pages > 0 ? p.pages : 1)};
+    const cuuint64_t cdims[3] = {(cuuint64_t)kWidth, (cuuint64_t)p.page_size, (cuuint64_t)p.pages};
     const cuuint64_t cstrides[2] = {(cuuint64_t)p.cache_stride[1] * 2, (cuuint64_t)p.cache_stride[0] * 2};
     const cuuint32_t cbox[3] = {64u, (cuuint32_t)a.box, 1u};
-    if (!encode_bf16_map(&maps.q, 3, p.q, qdims, qstrides, qbox) || !encode_bf16_map(&maps.cache, 3, p.cache, cdims, cstrides, cbox))
-        return FKDA_ERR_LAUNCH;
+    if (!encode_bf16_map(&maps.q, 3, p.q, qdims, qstrides, qbox)) return FKDA_ERR_LAUNCH;
+    maps.cache = maps.q;   // (where there is no page, nothing is read)
+    if (p.pages > 0 && p.max_pages > 0 && !encode_bf16_map(&maps.cache, 3, p.cache, cdims, cstrides, cbox)) return FKDA_ERR_LAUNCH;
     const int ctas = a.row_tiles * a.groups;
     const int rows_each = p.B * a.R > 4 * device_sm_count() ? 4 : 1, per = (a.R + rows_each - 1) / rows_each;
     const int64_t joins = p.B * per;

@@ -24,7 +24,7 @@ bool tile_strides(int64_t* stride, std::initializer_list<int64_t> sizes) {
 bool row_strides(const int64_t* stride, std::initializer_list<int64_t> sizes) {
     int i = 0;
     for (const int64_t n : sizes) {
-        if (n > 1 && stride[i] % 8 != 0) return false;
+        if (n > 1 && (stride[i] <= 0 || stride[i] % 8 != 0)) return false;
         ++i;
     }
     return true;
