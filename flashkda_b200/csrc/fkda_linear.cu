@@ -722,7 +722,7 @@ Segments plan(const fkda_linear_params& p) {
     const bool packed = p.cu_seqlens != nullptr;
     const int64_t rows = sms / p.H - (packed ? p.N : 0);   // (every packed sequence has one that is not full)
     const int64_t pieces = packed ? rows : rows / p.N, tokens = p.T;
-    if (pieces < 2 || p.N > 64) return none;
+    if (pieces < 2 || p.N > 64 || tokens == 0) return none;
     const int64_t len = ((tokens + pieces - 1) / pieces + kC - 1) / kC * kC;
     const int64_t segs = (tokens + len - 1) / len;
     if (segs < 2) return none;

@@ -52,6 +52,24 @@ def test_nothing_to_do_launches_nothing():
     assert L.fkda_linear_attention_fwd(params(T=0), None) == 0 and L.fkda_last_launch_count() == 0
 
 
+@pytest.mark.parametrize("B,T,H,N,packed", [(1, 0, 1, 1, False), (1, 0, 1, 3, True), (3, 0, 2, 3, False), (1, 1, 1, 1, False), (1, 1, 200, 1, False), (1, 10 ** 9, 1, 1, False),
+                                            (1, 10 ** 9, 1, 64, True), (64, 10 ** 6, 2, 64, False), (1, 5, 2, 10, True)])
+def test_workspace_size_of_any_call(B, T, H, N, packed):
+    size = flashkda_b200.linear_attention_workspace_size(B, T, H, N, packed)
+    rows = 148 + 2 * N     # segments that all SMs together walk, and the packed sequences' last ones
+    assert 0 <= size <= rows * H * (128 * 128 + 1) * 4
+    if T < 64 * 10:
+        assert size == 0
+
+
+def test_workspace_size_of_a_latent_step():
+    assert flashkda_b200.latent_decode_workspace_size(0, 1, 4) == 0
+    for B, Tq, H in ((1, 1, 1), (3, 4, 128), (36864, 1, 64)):
+        tiles = -(-Tq * H // 64)
+        size = flashkda_b200.latent_decode_workspace_size(B, Tq, H)
+        assert size % 4 == 0 and size <= max(148, tiles) * 2 * 64 * 513 * 4 + 16 * B
+
+
 # ---------------------------------------------------------------------------------------------------------- on the GPU
 @gpu
 @pytest.mark.parametrize("T", [1, 2, 15, 63, 64, 65, 127, 128, 129, 200])
