@@ -13,6 +13,11 @@
 // 512 dimensions x 64 rows as four accumulators of 128 lanes x 64 columns, so that the cache tile serves as the A operand for the
 // value product as it lies (dimension-major), and 256 of the 512 tensor-memory columns are enough.
 //
+// Measured: a tile of 64 tokens takes a CTA some 2 300 cycles of products (36 of 64 x 64 at 42, 16 of 128 x 64 at 49) and 1 100 of weights,
+// which run beside the next tile's scores, against 3 100 for its bytes: 64 sequences of 4 000 tokens of 64 heads walk at the copy
+// bandwidth; the listed batch of 128 uneven ones takes 153 to 172 us with its start, its outputs and the joining (0.64 to 0.57 of the copy
+// bandwidth).  384 rows per token: 321 to 340 us, 0.42 of cuBLAS.  One sequence of 2 989 tokens: 14 us, of which 6.5 are the walk.
+//
 // Numerics: as in the expanded form (fp32 scores, sums and outputs; weights against a reference within 2^8 of the running maximum,
 // rounded to bf16 for the value product only); parts are joined in fp32 in the order of the tokens.
 #include <algorithm>

@@ -2,19 +2,27 @@
 //     S_t = exp(g_t) S_{t-1} + v_t k_t^T  ([V, K]),   o_t = scale S_t q_t
 //
 // Prompts go through chunks of 64 tokens.  With G the running sum of g in a chunk and S the state in front of it,
-//     O = scale (P V + diag(exp(G)) Q S^T),   P_ij = exp(G_i - G_j) (q_i . k_j) for j <= i
-//     S' = exp(G_64) S + (diag(w) V)^T K,     w_j = exp(G_64 - G_j)
-// All four products run on tcgen05: q k^T and the two of O as accumulators of 64 rows, the state as one of 128 x 128 that stays in
-// tensor memory for the whole sequence.  The call is bound by HBM (1 KB per token and head against 2 x 128 x (64 + 128 + 128)
-// operations), so one CTA walks a (sequence, head) chain with everything between the copies in and out on the chip, and a chunk's
-// stages are spread over warpgroups: state (read, rounded for Q S^T, decayed, written back), scores and outputs, weighted
-// values, one warp each for the copies, the products and the decays.
+//     O^T = scale (V^T P^T + S Q^T diag(exp(G))),   P_ij = exp(G_i - G_j) (q_i . k_j) for j <= i
+//     S' = exp(G_64) S + (diag(w) V)^T K,           w_j = exp(G_64 - G_j)
+// The call is bound by HBM (1 KB per token and head against 2 x 128 x (64 + 128 + 128) operations), so one CTA walks a (sequence,
+// head) chain with everything between the copies in and out on the chip.  All products but q k^T have 128 rows (dimensions of v) on
+// tcgen05: the fp32 state stays in tensor memory for the whole sequence, and what multiplies k and q there (weighted values, a bf16 copy
+// of the state) is written to tensor memory as well, not through shared memory, whose bandwidth an earlier form with 64-row products
+// ran out of.  A chunk's stages are spread over warpgroups: state (read, decayed, copied; in two halves, one of which is decayed
+// while the other is updated), weights, outputs (two), weighted values (two), and a warp each for copies, two kinds of products and
+// decays.  Seven warps per scheduler want small code: roles that were unrolled waited for instructions 44 % of the time, 3.4 us per chunk
+// against 1.5 (96 chains) now.
+// Measured: 148 chains of 8 192 tokens 236 us, 5.3 TB/s (0.80 of the copy bandwidth); 8 x 16 384 tokens of 64 heads (512 chains: 3.46 rounds
+// of SMs, four are run) 1.66 ms, 2.02 where the power cap holds the clock at 1.6 GHz; a chain alone 1.5 us per chunk, which is the loop
+// from one update of the state to the next.  Few long chains are cut into segments (see plan()): 32 chains of 8 192 tokens 104 us, in one
+// piece 205.
 //
 // Numerics: decays are sums of g in fp32 over at most 64 tokens, w as sums over the tokens behind j (no differences of large sums).
 // P and the copy of S that Q multiplies are rounded to bf16, which the bf16 outputs do not show.  The state is not rounded: it
-// is fp32 throughout, and w V enters the product as three bf16 terms, which hold all 24 bits.
+// is fp32 throughout, and w V enters the product as three bf16 terms, which hold all 24 bits (two would do for 17: 3e-6 off).
 //
-// Single tokens: a read-modify-write of the state by a kernel of its own, as bound by HBM as that is.
+// Single tokens: a read-modify-write of the state by a kernel of its own, as bound by HBM as that is (256 x 64 states in bf16: 172 to
+// 190 us, 0.97 to 0.87 of the copy bandwidth; one sequence: the launch, 2.6 to 3.2 us).
 #include "fkda_tc5.cuh"
 
 namespace fkda {

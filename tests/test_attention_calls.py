@@ -207,6 +207,24 @@ def test_the_same_page_in_many_rows_of_the_table():
         assert_within(out[b], want, bound, f"sequence {b}")
 
 
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+def test_no_tokens_at_all(packed, kind):
+    """The state goes through, and becomes zero where none comes in."""
+    e = lambda *s: torch.empty(*s, device="cuda").bfloat16()
+    n = 3
+    h0 = torch.randn(n, 2, 128, 128, device="cuda").to(kind)
+    hT = torch.full_like(h0, 7.0)
+    B = 1 if packed else n
+    cu = torch.zeros(n + 1, dtype=torch.int64, device="cuda") if packed else None
+    args = e(B, 0, 2, 128), e(B, 0, 2, 128), e(B, 0, 2, 128), torch.empty(B, 0, 2, device="cuda"), 1.0, e(B, 0, 2, 128)
+    lib.linear_attention_fwd(*args, h0, hT, cu)
+    assert torch.equal(hT, h0)
+    lib.linear_attention_fwd(*args, None, hT, cu)
+    assert bool((hT == 0).all())
+    lib.latent_attention_fwd(e(B, 0, 2, 192), e(B, 0, 2, 128), e(B, 0, 64), e(B, 0, 2, 128), 1.0, e(B, 0, 2, 128), None, cu, cu)
+
+
 def test_decays_broadcast_over_tokens_or_heads():
     d = linear_inputs([130], 4, seed=7)
     for g in (-torch.rand(1, 1, 4, device="cuda").expand(1, 130, 4), -torch.rand(1, 130, 1, device="cuda").expand(1, 130, 4)):
