@@ -19,7 +19,8 @@
 //
 // Numerics: decays are sums of g in fp32 over at most 64 tokens, w as sums over the tokens behind j (no differences of large sums).
 // P and the copy of S that Q multiplies are rounded to bf16, which the bf16 outputs do not show.  The state is not rounded: it
-// is fp32 throughout, and w V enters the product as three bf16 terms, which hold all 24 bits (two would do for 17: 3e-6 off).
+// is fp32 throughout, and w V enters the product as three bf16 terms, which hold all 24 bits; as two, which hold 16, where the call's
+// states are bf16 (half a step of theirs is 2^-8, of the terms 2^-16; 6 % less time where the power cap rules).
 //
 // Single tokens: a read-modify-write of the state by a kernel of its own, as bound by HBM as that is (256 x 64 states in bf16: 172 to
 // 190 us, 0.97 to 0.87 of the copy bandwidth; one sequence: the launch, 2.6 to 3.2 us).
@@ -35,7 +36,6 @@ constexpr int kTileBytes = kC * 128;          // 64 tokens x 64 dimensions
 constexpr int kOperandBytes = 2 * kTileBytes; // a chunk of q, k or v
 constexpr int kStageBytes = 3 * kOperandBytes;
 constexpr int kStages = 3;
-constexpr int kTerms = 3;
 constexpr int kThreads = 896;                 // warpgroups: one each for state and scores, two each for outputs and values; copies, products, decays
 constexpr int kOffP = kStages * kStageBytes;
 constexpr int kOffOut = kOffP + 2 * kTileBytes;
@@ -192,8 +192,8 @@ __device__ __forceinline__ void store_state32(void* to, bool fp32, int64_t at, c
 }
 
 // kStates: only the state that each segment but the last leaves behind a zero one (the first: behind the initial state), and the
-// product of its decays.
-template <bool kStates>
+// product of its decays.  kTerms: of the weighted values, 2 where the call's states are bf16, else 3.
+template <bool kStates, int kTerms>
 __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_constant__ LinearArgs a, const __grid_constant__ LinearMaps maps) {
     extern __shared__ __align__(1024) uint8_t smem[];
     Bars& bar = *reinterpret_cast<Bars*>(smem + kOffBars);
@@ -579,8 +579,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
                         mul2(x, y, i < 2 ? w0[0] : w1[0], i < 2 ? w0[1] : w1[1]);
 #pragma unroll
                         for (int m = 0; m < kTerms; ++m) {
-                            // the upper 16 bits of what is left, which are a bf16: after three times nothing is
-                            term[b][d][m][i] = __byte_perm(x, y, 0x7632);
+                            // the upper 16 bits of what is left, which are a bf16 (after three times nothing is left); the last one rounded
+                            term[b][d][m][i] = m + 1 < kTerms ? __byte_perm(x, y, 0x7632) : pack_bf2(f(x), f(y));
                             if (m + 1 < kTerms) sub2(x, y, x & 0xffff0000u, y & 0xffff0000u);
                         }
                     }
@@ -718,6 +718,12 @@ __global__ void __launch_bounds__(256) linear_carry_kernel(const __grid_constant
     }
 }
 
+template <bool kStates, int kTerms>
+bool launch_walk(int64_t ctas, cudaStream_t stream, const LinearArgs& a, const LinearMaps& maps) {
+    constexpr auto kKernel = linear_chunk_kernel<kStates, kTerms>;
+    return allow_smem<kKernel>(kSmem) && launch_dependent(kKernel, ctas, kThreads, kSmem, stream, a, maps);
+}
+
 // Tokens of a segment, 0 for none, and how many (sequence, segment) rows there are at most.  Segments put the idle SMs of few long
 // chains to work, for half of a chunk's work more: the states are made first, without outputs.
 struct Segments {
@@ -801,15 +807,18 @@ int launch_linear(const fkda_linear_params& p, cudaStream_t stream, int* n_launc
         a.seg_decay = a.seg_state + seg.rows * p.H * (kD * kD);
         // the longest first where not all run at once
         a.ordered = p.cu_seqlens != nullptr && seg.len == 0 && p.N > 1 && p.N <= kThreads && chains > device_sm_count();
-        if (!allow_smem<linear_chunk_kernel<false>>(kSmem)) return FKDA_ERR_LAUNCH;
+        // (outputs do not depend on whether a final state is asked for)
+        const bool exact = a.state_fp32 || (p.initial_state == nullptr && p.final_state == nullptr);
+        auto walk = [&](bool states) {
+            const int64_t ctas = seg.rows * p.H;
+            if (states) return exact ? launch_walk<true, 3>(ctas, stream, a, maps) : launch_walk<true, 2>(ctas, stream, a, maps);
+            return exact ? launch_walk<false, 3>(ctas, stream, a, maps) : launch_walk<false, 2>(ctas, stream, a, maps);
+        };
         if (seg.len > 0) {
-            if (!allow_smem<linear_chunk_kernel<true>>(kSmem)) return FKDA_ERR_LAUNCH;
-            if (!launch_dependent(linear_chunk_kernel<true>, seg.rows * p.H, kThreads, kSmem, stream, a, maps) ||
-                !launch_dependent(linear_carry_kernel, chains * 16, 256, 0, stream, a))
-                return FKDA_ERR_LAUNCH;
+            if (!walk(true) || !launch_dependent(linear_carry_kernel, chains * 16, 256, 0, stream, a)) return FKDA_ERR_LAUNCH;
             launches += 2;
         }
-        if (!launch_dependent(linear_chunk_kernel<false>, seg.rows * p.H, kThreads, kSmem, stream, a, maps)) return FKDA_ERR_LAUNCH;
+        if (!walk(false)) return FKDA_ERR_LAUNCH;
         ++launches;
     }
     *n_launches = launches;

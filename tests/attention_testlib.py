@@ -37,8 +37,12 @@ def linear_oracle(q, k, v, g, scale, h0=None):
 
 
 def state_bound(T, size, S, dtype):
-    """fp32 products of terms that hold 24 bits: a chunk adds at most 16 partial sums, each off by 2^-23 of the magnitudes."""
-    return size * (T // 64 + 2) * 16 * 2.0 ** -23 + 1e-30 + (S.abs() * BF if dtype == torch.bfloat16 else 0)
+    """fp32 products of terms that hold 24 bits: a chunk adds at most 16 partial sums, each off by 2^-23 of the magnitudes.  A state that
+    leaves in bf16 is made of weighted values in two bf16 terms: the first is x cut off behind 8 bits, which leaves less than 2^(e-7) for
+    2^e <= |x|, and the second that rounded to 8 bits, off by at most half of 2^-7 of a number below 2^(e-7), whose leading bit is at most
+    2^(e-8): 2^-8 2^(e-8) <= 2^-16 |x|."""
+    terms = 2.0 ** -16 if dtype == torch.bfloat16 else 0.0
+    return size * ((T // 64 + 2) * 16 * 2.0 ** -23 + terms) + 1e-30 + (S.abs() * BF if dtype == torch.bfloat16 else 0)
 
 
 def softmax_oracle(scores, values, magnitude):
