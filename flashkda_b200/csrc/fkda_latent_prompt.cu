@@ -54,7 +54,8 @@ struct PromptArgs {
 
 constexpr int kMaxOrdered = 512;             // packed sequences that are taken in the order of their keys
 struct Bars {
-    uint64_t q_full, full[kSlots], empty[kSlots], s_full[2], p_full[2][2], o_done[2], drained;
+    // (keys and values of block i: the barriers i & 1)
+    uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2][2], o_done[2], drained;
     uint32_t tmem;
     int abort;
     int order[kMaxOrdered];
@@ -145,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         mbar_init(&bar.q_full, 1);
-        for (int i = 0; i < kSlots; ++i) mbar_init(&bar.full[i], 1), mbar_init(&bar.empty[i], 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&bar.k_full[i], 1), mbar_init(&bar.v_full[i], 1), mbar_init(&bar.k_empty[i], 1), mbar_init(&bar.v_empty[i], 1);
         for (int i = 0; i < 2; ++i) mbar_init(&bar.s_full[i], 1), mbar_init(&bar.p_full[i][0], kTile), mbar_init(&bar.p_full[i][1], kTile), mbar_init(&bar.o_done[i], 1);
         mbar_init(&bar.drained, 1);
         bar.abort = 0;
@@ -185,31 +186,40 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
         if (blocks > 0) {
             const uint32_t q_addr = smem_u32(q_smem), ring_addr = smem_u32(ring), leader = elect_one();
             const int q0 = uniform((int)(p.q0 + p.row0)), row = uniform((int)p.b), k0 = uniform((int)p.k0);
-            expect(&bar.q_full, 2 * kKeyTiles * kSlotBytes, leader);
+            // Block i's five tiles follow one another in the ring of eight: its keys take the places of the last keys and the values of
+            // block i - 2, its values those of the first keys of block i - 1.
+            int keys = 0, values = 0;   // blocks of either that have been asked for
+            auto empty = [&](uint64_t* b, int phase) { return __all_sync(0xffffffffu, wait(b, phase & 1, &bar.abort)) != 0; };
+            auto slot = [&](int s) { return ring_addr + (s % kSlots) * kSlotBytes; };
 #pragma unroll 1
-            for (int w = 0; w < 2; ++w)
-#pragma unroll
-                for (int c = 0; c < kKeyTiles; ++c) load_4d(q_addr + (w * kKeyTiles + c) * kSlotBytes, &maps.q, c * 64, h, q0 + w * kTile, row, &bar.q_full, leader);
-            int s = 0;
-            bool ok = true;
+            for (int i = 0; i < blocks; ++i) {
+                const int t = k0 + i * kTile, s = i * (kKeyTiles + kValueTiles);
+                if (i >= 2 && !empty(&bar.v_empty[i & 1], (i >> 1) - 1)) break;   // (the keys of block i - 2 were waited for below)
+                uint64_t* full = &bar.k_full[i & 1];
+                expect(full, kKeyTiles * kSlotBytes, leader);
+                load_4d(slot(s), &maps.k, 0, h, t, row, full, leader);
+                load_4d(slot(s + 1), &maps.k, 64, h, t, row, full, leader);
+                load_3d(slot(s + 2), &maps.r, 0, t, row, full, leader);
+                ++keys;
+                if (i == 0) {
+                    expect(&bar.q_full, 2 * kKeyTiles * kSlotBytes, leader);
 #pragma unroll 1
-            for (int i = 0; i < blocks && ok; ++i) {
-                const int t = k0 + i * kTile;
+                    for (int w = 0; w < 2; ++w)
 #pragma unroll
-                for (int c = 0; c < kKeyTiles + kValueTiles; ++c, ++s) {
-                    const int slot = s % kSlots;
-                    if (s >= kSlots) ok = __all_sync(0xffffffffu, wait(&bar.empty[slot], (s / kSlots - 1) & 1, &bar.abort));
-                    if (!ok) break;
-                    const uint32_t dst = ring_addr + slot * kSlotBytes;
-                    expect(&bar.full[slot], kSlotBytes, leader);
-                    if (c < 2) load_4d(dst, &maps.k, c * 64, h, t, row, &bar.full[slot], leader);
-                    else if (c == 2) load_3d(dst, &maps.r, 0, t, row, &bar.full[slot], leader);
-                    else load_4d(dst, &maps.v, (c - 3) * 64, h, t, row, &bar.full[slot], leader);
+                        for (int c = 0; c < kKeyTiles; ++c) load_4d(q_addr + (w * kKeyTiles + c) * kSlotBytes, &maps.q, c * 64, h, q0 + w * kTile, row, &bar.q_full, leader);
                 }
+                if (i >= 1 && !empty(&bar.k_empty[(i - 1) & 1], (i - 1) >> 1)) break;
+                full = &bar.v_full[i & 1];
+                expect(full, kValueTiles * kSlotBytes, leader);
+                load_4d(slot(s + 3), &maps.v, 0, h, t, row, full, leader);
+                load_4d(slot(s + 4), &maps.v, 64, h, t, row, full, leader);
+                ++values;
             }
             drain(&bar.q_full, 0);
 #pragma unroll 1
-            for (int k = max(0, s - kSlots); k < s; ++k) drain(&bar.full[k % kSlots], (k / kSlots) & 1);
+            for (int i = max(0, keys - 2); i < keys; ++i) drain(&bar.k_full[i & 1], (i >> 1) & 1);
+#pragma unroll 1
+            for (int i = max(0, values - 2); i < values; ++i) drain(&bar.v_full[i & 1], (i >> 1) & 1);
             __syncwarp();
         }
     } else if (warp == 9) {
@@ -223,8 +233,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
 #pragma unroll
                 for (int c = 0; c < kKeyTiles; ++c) {
                     const int s = i * kEach + c;
-                    if (first) wait_warp(&bar.full[s % kSlots], (s / kSlots) & 1, &bar.abort);
-                    fence_after();
+                    if (first && c == 0) wait_warp(&bar.k_full[i & 1], (i >> 1) & 1, &bar.abort);
+                    if (c == 0) fence_after();
                     const uint32_t k_desc = ring_desc + (s % kSlots) * (kSlotBytes / 16);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
@@ -232,13 +242,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
                 }
                 commit(&bar.s_full[w], leader);
             };
-            auto free_slots = [&](int first, int count) {
-                for (int s = first; s < first + count; ++s) commit(&bar.empty[s % kSlots], leader);
-            };
 #pragma unroll
             for (int w = 0; w < 2; ++w)
                 if (n[w] > 0) scores(w, 0, w == 0 || n[0] == 0);
-            free_slots(0, kKeyTiles);
+            commit(&bar.k_empty[0], leader);
 #pragma unroll 1
             for (int i = 0; i < blocks; ++i) {
                 const int first_v = i < n[0] ? 0 : 1, last_v = i < n[1] ? 1 : 0;
@@ -249,8 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {   // 64 keys
                         wait_warp(&bar.p_full[w][half], i & 1, &bar.abort);
-                        if (half == 0 && w == first_v)
-                            for (int s = i * kEach + kKeyTiles; s < (i + 1) * kEach; ++s) wait_warp(&bar.full[s % kSlots], (s / kSlots) & 1, &bar.abort);
+                        if (half == 0 && w == first_v) wait_warp(&bar.v_full[i & 1], (i >> 1) & 1, &bar.abort);
                         fence_after();
 #pragma unroll
                         for (int c = 0; c < kValueTiles; ++c) {   // 64 dimensions at a time: the two tiles need not be neighbours in the ring
@@ -261,10 +267,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
                         }
                     }
                     commit(&bar.o_done[w], leader);
-                    if (w == last_v) free_slots(i * kEach + kKeyTiles, kValueTiles);
+                    if (w == last_v) commit(&bar.v_empty[i & 1], leader);
                     if (i + 1 < n[w]) {
                         scores(w, i + 1, w == first_k);
-                        if (w == last_k) free_slots((i + 1) * kEach, kKeyTiles);
+                        if (w == last_k) commit(&bar.k_empty[(i + 1) & 1], leader);
                     }
                 }
             }
@@ -324,9 +330,9 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
             // values behind the sequence's last key are another sequence's, or nobody's: nothing times them must be nothing
             if ((i + 1) * kTile > p.len_k && w == (i < n0 ? 0 : 1)) {
                 const int from = p.len_k - i * kTile;
+                wait_warp(&bar.v_full[i & 1], (i >> 1) & 1, &bar.abort);
                 for (int v = 0; v < kValueTiles; ++v) {
                     const int sl = i * (kKeyTiles + kValueTiles) + kKeyTiles + v;
-                    wait_warp(&bar.full[sl % kSlots], (sl / kSlots) & 1, &bar.abort);
                     uint4* dst = reinterpret_cast<uint4*>(ring + (sl % kSlots) * kSlotBytes);
                     for (int k = from * 8 + (threadIdx.x & 127); k < kTile * 8; k += 128) dst[k] = make_uint4(0, 0, 0, 0);
                 }
