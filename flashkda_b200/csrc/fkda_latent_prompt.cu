@@ -5,20 +5,22 @@
 // One pass over the keys with the running maximum and sum of the softmax.  A CTA serves 256 rows of one head as two tiles of
 // 128, each with a warpgroup of its own that turns scores into weights, one row per thread; while one tile's weights are being made
 // the tensor cores work for the other.  Scores and outputs live in tensor memory (2 x 128 + 2 x 128 columns), the weights
-// overwrite the scores as the A operand of the product with v.  Keys and values come through a ring of eight 16 KB tiles
+// overwrite the scores as the A operand of the product with v.  Keys and values come through eight 16 KB tiles
 // (128 tokens x 64 dimensions); the rotated part needs no copy beside the others: it is the third tile of a key block, read
 // through a map of its own.  Packed sequences with more keys are taken first.
 //
-// Measured: 8 192 tokens of 32 heads 535 us, 1.28 PFLOP/s (0.77 of cuBLAS in a burst); 636 to 640 us, 0.78 of what cuBLAS sustains, where the
-// power cap holds the clock.  A block of keys keeps the tensor cores busy for 1 280 cycles per tile and the exponentials for 1 024, so
-// each tile's weights have to be made while the other's products run; what is left between them are the hand-overs (scores to
-// weights to product, some 500 cycles).  A row's 128 scores are held in registers (208 of them per thread): read in pieces of 64,
-// twice, the same call takes 546 us with less code.  A persistent form that loads the next item's keys beside the last one's outputs:
-// 546 to 610.
+// Measured: 8 192 tokens of 32 heads 516 us, 1.33 PFLOP/s (0.79 of cuBLAS in a burst); 595, 0.84 of what cuBLAS sustains, where the power
+// cap holds the clock.
+// A pair of tiles takes 3 160 cycles per block of keys, for 2 560 of tensor-core work and 2 048 of exponentials; a tile's own
+// chain, scores to weights (1 680) to product and the next scores (1 020), with 390 between them, is as long.  One thread's instruction
+// stream feeds the tensor cores, so what it has to do beside products counts: barriers per block instead of per 16 KB tile made
+// 541 us 520, one product for all 128 dimensions of the values instead of two another 5.  No gain: a quarter of the
+// exponentials as polynomials (530 to 539), weights handed over as 96 + 32 keys instead of 64 + 64 (516), scores read in two pieces of 64
+// with less code (546 for 541), a persistent form that loads the next item's keys beside the last one's outputs (546 to 610).
 //
 // Numerics: products of bf16 with fp32 sums, weights relative to a reference that follows the running maximum once that is
 // 2^8 above it (so weights stay below 2^8 and the sums are exact to 32 bits either way), weights rounded to bf16 for the product
-// with v (their relative error, 2^-9 at most, averages out over the keys; the sum and lse use the unrounded weights).
+// with v (their relative error, 2^-8 at most, averages out over the keys; the sum and lse use the unrounded weights).
 #define FKDA_WAITS_INLINE
 #include "fkda_tc5.cuh"
 
@@ -32,6 +34,11 @@ constexpr int kRows = 2 * kTile;             // query rows of a CTA
 constexpr int kSlotBytes = kTile * 128;      // 128 tokens x 64 dimensions
 constexpr int kSlots = 8;
 constexpr int kKeyTiles = 3, kValueTiles = 2;
+// Where block i's tiles lie: the keys' first two in one of three pairs of slots, where block i - 3's lay, block i - 2's values after
+// them; its values in the pair of block i - 1's keys; the keys' third tile in one of two more slots.  So the tiles of the values are
+// always neighbours (one product covers their 128 dimensions), and a block's keys wait for nothing younger than block i - 2.
+__device__ __forceinline__ int key_slot(int i, int c) { return c < 2 ? 2 * (i % 3) + c : 6 + (i & 1); }
+__device__ __forceinline__ int value_slot(int i) { return 2 * ((i + 2) % 3); }
 constexpr int kThreads = 384;                // two softmax warpgroups, and one with a loading and a multiplying warp
 // Registers of a thread: 168 at launch, then 208 for a row's 128 scores and what is made of them; 2 x 208 + 88 = 3 x 168
 constexpr int kRegsRow = 208, kRegsRest = 88;
@@ -186,20 +193,18 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
         if (blocks > 0) {
             const uint32_t q_addr = smem_u32(q_smem), ring_addr = smem_u32(ring), leader = elect_one();
             const int q0 = uniform((int)(p.q0 + p.row0)), row = uniform((int)p.b), k0 = uniform((int)p.k0);
-            // Block i's five tiles follow one another in the ring of eight: its keys take the places of the last keys and the values of
-            // block i - 2, its values those of the first keys of block i - 1.
             int keys = 0, values = 0;   // blocks of either that have been asked for
             auto empty = [&](uint64_t* b, int phase) { return __all_sync(0xffffffffu, wait(b, phase & 1, &bar.abort)) != 0; };
-            auto slot = [&](int s) { return ring_addr + (s % kSlots) * kSlotBytes; };
+            auto slot = [&](int s) { return ring_addr + s * kSlotBytes; };
 #pragma unroll 1
             for (int i = 0; i < blocks; ++i) {
-                const int t = k0 + i * kTile, s = i * (kKeyTiles + kValueTiles);
+                const int t = k0 + i * kTile;
                 if (i >= 2 && !empty(&bar.v_empty[i & 1], (i >> 1) - 1)) break;   // (the keys of block i - 2 were waited for below)
                 uint64_t* full = &bar.k_full[i & 1];
                 expect(full, kKeyTiles * kSlotBytes, leader);
-                load_4d(slot(s), &maps.k, 0, h, t, row, full, leader);
-                load_4d(slot(s + 1), &maps.k, 64, h, t, row, full, leader);
-                load_3d(slot(s + 2), &maps.r, 0, t, row, full, leader);
+                load_4d(slot(key_slot(i, 0)), &maps.k, 0, h, t, row, full, leader);
+                load_4d(slot(key_slot(i, 1)), &maps.k, 64, h, t, row, full, leader);
+                load_3d(slot(key_slot(i, 2)), &maps.r, 0, t, row, full, leader);
                 ++keys;
                 if (i == 0) {
                     expect(&bar.q_full, 2 * kKeyTiles * kSlotBytes, leader);
@@ -211,8 +216,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
                 if (i >= 1 && !empty(&bar.k_empty[(i - 1) & 1], (i - 1) >> 1)) break;
                 full = &bar.v_full[i & 1];
                 expect(full, kValueTiles * kSlotBytes, leader);
-                load_4d(slot(s + 3), &maps.v, 0, h, t, row, full, leader);
-                load_4d(slot(s + 4), &maps.v, 64, h, t, row, full, leader);
+                load_4d(slot(value_slot(i)), &maps.v, 0, h, t, row, full, leader);
+                load_4d(slot(value_slot(i) + 1), &maps.v, 64, h, t, row, full, leader);
                 ++values;
             }
             drain(&bar.q_full, 0);
@@ -225,17 +230,15 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
     } else if (warp == 9) {
         // ---- products ----
         if (blocks > 0) {
-            constexpr uint32_t kIdS = idesc(kTile, kTile, false, false), kIdO = idesc(kTile, 64, false, true);
-            const uint32_t q_desc = desc(smem_u32(q_smem)), ring_desc = desc(smem_u32(ring)), leader = elect_one();
-            constexpr int kEach = kKeyTiles + kValueTiles;
+            constexpr uint32_t kIdS = idesc(kTile, kTile, false, false), kIdO = idesc(kTile, 128, false, true);
+            const uint32_t q_desc = desc(smem_u32(q_smem)), k_desc0 = desc(smem_u32(ring)), v_desc0 = desc(smem_u32(ring), kSlotBytes), leader = elect_one();
             wait_warp(&bar.q_full, 0, &bar.abort);
             auto scores = [&](int w, int i, bool first) {   // tile w against key block i
 #pragma unroll
                 for (int c = 0; c < kKeyTiles; ++c) {
-                    const int s = i * kEach + c;
                     if (first && c == 0) wait_warp(&bar.k_full[i & 1], (i >> 1) & 1, &bar.abort);
                     if (c == 0) fence_after();
-                    const uint32_t k_desc = ring_desc + (s % kSlots) * (kSlotBytes / 16);
+                    const uint32_t k_desc = k_desc0 + key_slot(i, c) * (kSlotBytes / 16);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         mma_ss(tmem + kS + w * kTile, q_desc + ((w * kKeyTiles + c) * kSlotBytes + k * 32) / 16, k_desc + k * 32 / 16, kIdS, (c | k) != 0, leader);
@@ -258,13 +261,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
                         wait_warp(&bar.p_full[w][half], i & 1, &bar.abort);
                         if (half == 0 && w == first_v) wait_warp(&bar.v_full[i & 1], (i >> 1) & 1, &bar.abort);
                         fence_after();
+                        const uint32_t v_desc = v_desc0 + value_slot(i) * (kSlotBytes / 16);
 #pragma unroll
-                        for (int c = 0; c < kValueTiles; ++c) {   // 64 dimensions at a time: the two tiles need not be neighbours in the ring
-                            const uint32_t v_desc = ring_desc + ((i * kEach + kKeyTiles + c) % kSlots) * (kSlotBytes / 16);
-#pragma unroll
-                            for (int k = 4 * half; k < 4 * half + 4; ++k)
-                                mma_ts(tmem + kO + w * kTile + c * 64, tmem + kS + w * kTile + k * 8, v_desc + k * 2048 / 16, kIdO, i > 0 || k > 0, leader);
-                        }
+                        for (int k = 4 * half; k < 4 * half + 4; ++k)
+                            mma_ts(tmem + kO + w * kTile, tmem + kS + w * kTile + k * 8, v_desc + k * 2048 / 16, kIdO, i > 0 || k > 0, leader);
                     }
                     commit(&bar.o_done[w], leader);
                     if (w == last_v) commit(&bar.v_empty[i & 1], leader);
@@ -332,8 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
                 const int from = p.len_k - i * kTile;
                 wait_warp(&bar.v_full[i & 1], (i >> 1) & 1, &bar.abort);
                 for (int v = 0; v < kValueTiles; ++v) {
-                    const int sl = i * (kKeyTiles + kValueTiles) + kKeyTiles + v;
-                    uint4* dst = reinterpret_cast<uint4*>(ring + (sl % kSlots) * kSlotBytes);
+                    uint4* dst = reinterpret_cast<uint4*>(ring + (value_slot(i) + v) * kSlotBytes);
                     for (int k = from * 8 + (threadIdx.x & 127); k < kTile * 8; k += 128) dst[k] = make_uint4(0, 0, 0, 0);
                 }
                 fence_proxy_async_smem();

@@ -13,7 +13,7 @@
 // decays.  Seven warps per scheduler want small code: roles that were unrolled waited for instructions 44 % of the time, 3.4 us per chunk
 // against 1.5 (96 chains) now.
 // Measured: 148 chains of 8 192 tokens 236 us, 5.3 TB/s (0.80 of the copy bandwidth); 8 x 16 384 tokens of 64 heads (512 chains: 3.46 rounds
-// of SMs, four are run) 1.66 ms, 2.02 where the power cap holds the clock at 1.6 GHz; a chain alone 1.5 us per chunk, which is the loop
+// of SMs, four are run) 1.66 ms, 1.79 to 1.92 where the power cap holds the clock (1.6 to 1.75 GHz); a chain alone 1.5 us per chunk, which is the loop
 // from one update of the state to the next.  Few long chains are cut into segments (see plan()): 32 chains of 8 192 tokens 104 us, in one
 // piece 205.
 //
