@@ -16,7 +16,8 @@
 // stream feeds the tensor cores, so what it has to do beside products counts: barriers per block instead of per 16 KB tile made
 // 541 us 520, one product for all 128 dimensions of the values instead of two another 5.  No gain: a quarter of the
 // exponentials as polynomials (530 to 539), weights handed over as 96 + 32 keys instead of 64 + 64 (516), scores read in two pieces of 64
-// with less code (546 for 541), a persistent form that loads the next item's keys beside the last one's outputs (546 to 610).
+// with less code (546 for 541), outputs stored as whole rows by way of shared memory (513 to 516), a persistent form that loads the next item's keys beside the last one's outputs (546 to
+// 610).
 //
 // Numerics: products of bf16 with fp32 sums, weights relative to a reference that follows the running maximum once that is
 // 2^8 above it (so weights stay below 2^8 and the sums are exact to 32 bits either way), weights rounded to bf16 for the product
@@ -62,7 +63,7 @@ struct PromptArgs {
 constexpr int kMaxOrdered = 512;             // packed sequences that are taken in the order of their keys
 struct Bars {
     // (keys and values of block i: the barriers i & 1)
-    uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2][2], o_done[2], drained;
+    uint64_t q_full[2], k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2][2], o_done[2], drained;
     uint32_t tmem;
     int abort;
     int order[kMaxOrdered];
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
     Bars& bar = *reinterpret_cast<Bars*>(ring + kSlots * kSlotBytes);
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        mbar_init(&bar.q_full, 1);
+        mbar_init(&bar.q_full[0], 1), mbar_init(&bar.q_full[1], 1);
         for (int i = 0; i < 2; ++i) mbar_init(&bar.k_full[i], 1), mbar_init(&bar.v_full[i], 1), mbar_init(&bar.k_empty[i], 1), mbar_init(&bar.v_empty[i], 1);
         for (int i = 0; i < 2; ++i) mbar_init(&bar.s_full[i], 1), mbar_init(&bar.p_full[i][0], kTile), mbar_init(&bar.p_full[i][1], kTile), mbar_init(&bar.o_done[i], 1);
         mbar_init(&bar.drained, 1);
@@ -207,11 +208,12 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
                 load_3d(slot(key_slot(i, 2)), &maps.r, 0, t, row, full, leader);
                 ++keys;
                 if (i == 0) {
-                    expect(&bar.q_full, 2 * kKeyTiles * kSlotBytes, leader);
 #pragma unroll 1
-                    for (int w = 0; w < 2; ++w)
+                    for (int w = 0; w < 2; ++w) {
+                        expect(&bar.q_full[w], kKeyTiles * kSlotBytes, leader);
 #pragma unroll
-                        for (int c = 0; c < kKeyTiles; ++c) load_4d(q_addr + (w * kKeyTiles + c) * kSlotBytes, &maps.q, c * 64, h, q0 + w * kTile, row, &bar.q_full, leader);
+                        for (int c = 0; c < kKeyTiles; ++c) load_4d(q_addr + (w * kKeyTiles + c) * kSlotBytes, &maps.q, c * 64, h, q0 + w * kTile, row, &bar.q_full[w], leader);
+                    }
                 }
                 if (i >= 1 && !empty(&bar.k_empty[(i - 1) & 1], (i - 1) >> 1)) break;
                 full = &bar.v_full[i & 1];
@@ -220,7 +222,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
                 load_4d(slot(value_slot(i) + 1), &maps.v, 64, h, t, row, full, leader);
                 ++values;
             }
-            drain(&bar.q_full, 0);
+            drain(&bar.q_full[0], 0);
+            drain(&bar.q_full[1], 0);
 #pragma unroll 1
             for (int i = max(0, keys - 2); i < keys; ++i) drain(&bar.k_full[i & 1], (i >> 1) & 1);
 #pragma unroll 1
@@ -232,7 +235,6 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
         if (blocks > 0) {
             constexpr uint32_t kIdS = idesc(kTile, kTile, false, false), kIdO = idesc(kTile, 128, false, true);
             const uint32_t q_desc = desc(smem_u32(q_smem)), k_desc0 = desc(smem_u32(ring)), v_desc0 = desc(smem_u32(ring), kSlotBytes), leader = elect_one();
-            wait_warp(&bar.q_full, 0, &bar.abort);
             auto scores = [&](int w, int i, bool first) {   // tile w against key block i
 #pragma unroll
                 for (int c = 0; c < kKeyTiles; ++c) {
@@ -247,7 +249,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
             };
 #pragma unroll
             for (int w = 0; w < 2; ++w)
-                if (n[w] > 0) scores(w, 0, w == 0 || n[0] == 0);
+                if (n[w] > 0) {
+                    wait_warp(&bar.q_full[w], 0, &bar.abort);
+                    scores(w, 0, w == 0 || n[0] == 0);
+                }
             commit(&bar.k_empty[0], leader);
 #pragma unroll 1
             for (int i = 0; i < blocks; ++i) {
