@@ -16,8 +16,8 @@
 // stream feeds the tensor cores, so what it has to do beside products counts: barriers per block instead of per 16 KB tile made
 // 541 us 520, one product for all 128 dimensions of the values instead of two another 5.  No gain: a quarter of the
 // exponentials as polynomials (530 to 539), weights handed over as 96 + 32 keys instead of 64 + 64 (516), scores read in two pieces of 64
-// with less code (546 for 541), outputs stored as whole rows by way of shared memory (513 to 516), a persistent form that loads the next item's keys beside the last one's outputs (546 to
-// 610).
+// with less code (546 for 541), outputs stored as whole rows by way of shared memory (513 to 516), a persistent form that loads
+// the next item's keys beside the last one's outputs (546 to 610).
 //
 // Numerics: products of bf16 with fp32 sums, weights relative to a reference that follows the running maximum once that is
 // 2^8 above it (so weights stay below 2^8 and the sums are exact to 32 bits either way), weights rounded to bf16 for the product
