@@ -45,8 +45,9 @@ def linear_attention_fwd(q, k, v, g, scale, out, initial_state=None, final_state
     (then ``B`` must be 1).  Rows of ``out`` that no sequence has are left as they were.
 
     Sequences of more than one token go through 64-token chunks on the tensor cores; single tokens (``T == 1``, or the sequences of one
-    token in a packed batch of mostly such) through one read-modify-write of the states.  The state is fp32 throughout, whatever its
-    type in memory.  ``workspace``: optional caller-owned uint8 scratch for calls that need some
+    token in a packed batch of mostly such) through one read-modify-write of the states.  In between the state is fp32, whatever its type
+    in memory; what a chunk adds to it holds 24 bits, or 16 behind a bf16 ``initial_state``.  Outputs do not depend on whether a
+    ``final_state`` is asked for, nor on its type.  ``workspace``: optional caller-owned uint8 scratch for calls that need some
     (``linear_attention_workspace_size``).
     """
     _linear_attention_fwd(q, k, v, g, scale, out, initial_state, final_state, cu_seqlens, workspace)

@@ -19,8 +19,8 @@
 //
 // Numerics: decays are sums of g in fp32 over at most 64 tokens, w as sums over the tokens behind j (no differences of large sums).
 // P and the copy of S that Q multiplies are rounded to bf16, which the bf16 outputs do not show.  The state is not rounded: it
-// is fp32 throughout, and w V enters the product as three bf16 terms, which hold all 24 bits; as two, which hold 16, where the call's
-// states are bf16 (half a step of theirs is 2^-8, of the terms 2^-16; 6 % less time where the power cap rules).
+// is fp32 throughout, and w V enters the product as three bf16 terms, which hold all 24 bits; as two, which hold 16, where the
+// initial state is bf16 (half a step of its own is 2^-8, of the terms 2^-16; 6 % less time where the power cap rules).
 //
 // Single tokens: a read-modify-write of the state by a kernel of its own, as bound by HBM as that is (256 x 64 states in bf16: 172 to
 // 190 us, 0.97 to 0.87 of the copy bandwidth; one sequence: the launch, 2.6 to 3.2 us).
@@ -192,7 +192,7 @@ __device__ __forceinline__ void store_state32(void* to, bool fp32, int64_t at, c
 }
 
 // kStates: only the state that each segment but the last leaves behind a zero one (the first: behind the initial state), and the
-// product of its decays.  kTerms: of the weighted values, 2 where the call's states are bf16, else 3.
+// product of its decays.  kTerms: of the weighted values, 2 where the initial state is bf16, else 3.
 template <bool kStates, int kTerms>
 __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_constant__ LinearArgs a, const __grid_constant__ LinearMaps maps) {
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -807,8 +807,8 @@ int launch_linear(const fkda_linear_params& p, cudaStream_t stream, int* n_launc
         a.seg_decay = a.seg_state + seg.rows * p.H * (kD * kD);
         // the longest first where not all run at once
         a.ordered = p.cu_seqlens != nullptr && seg.len == 0 && p.N > 1 && p.N <= kThreads && chains > device_sm_count();
-        // (outputs do not depend on whether a final state is asked for)
-        const bool exact = a.state_fp32 || (p.initial_state == nullptr && p.final_state == nullptr);
+        // (by the initial state alone: outputs do not depend on whether, and in which type, a final state is asked for)
+        const bool exact = a.state_fp32 || p.initial_state == nullptr;
         auto walk = [&](bool states) {
             const int64_t ctas = seg.rows * p.H;
             if (states) return exact ? launch_walk<true, 3>(ctas, stream, a, maps) : launch_walk<true, 2>(ctas, stream, a, maps);
