@@ -59,3 +59,28 @@ def test_outputs_do_not_depend_on_the_final_state(lens, H, first):
     for n, T in enumerate(lens):
         check_head(d, n, at, T, H - 1, h0, finals[1], packed)
         at += T
+
+
+def microseconds(call, calls=20):
+    best = []
+    for _ in range(5):
+        torch.cuda.synchronize()
+        start, end = torch.cuda.Event(True), torch.cuda.Event(True)
+        start.record()
+        for _ in range(calls):
+            call()
+        end.record()
+        end.synchronize()
+        best.append(start.elapsed_time(end) / calls * 1e3)
+    return min(best[1:])
+
+
+@pytest.mark.parametrize("n,T,H", [(256, 20, 4), (800, 20, 4)])
+def test_many_short_packed_sequences_cost_what_a_fixed_batch_costs(n, T, H):
+    """Their chains are walked in the same way, so nothing may be looked up on the way that takes as long (half as much again is left)."""
+    times = []
+    for packed in (False, True):
+        d = linear_inputs([T] * n, H, packed=packed)
+        hT = torch.zeros_like(d["h0"])
+        times.append(microseconds(lambda: call(d, d["h0"], hT)))
+    assert times[1] < 1.5 * times[0], times
