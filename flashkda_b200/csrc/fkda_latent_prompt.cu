@@ -55,12 +55,12 @@ struct PromptArgs {
     const int64_t *cu_q, *cu_k;
     int64_t B, T, Tk, N, out_batch, out_token, out_head;
     int H;
-    uint32_t sms;
+    bool ordered;          // packed sequences: those with more keys first
     float scale;
     int causal;
 };
 
-constexpr int kMaxOrdered = 512;             // packed sequences that are taken in the order of their keys
+constexpr int kMaxOrdered = 32;              // packed sequences that are taken in the order of their keys
 struct Bars {
     // (keys and values of block i: the barriers i & 1)
     uint64_t q_full[2], k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2][2], o_done[2], drained;
@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
     fence_after();
     constexpr uint32_t tmem = 0;   // (all columns are this CTA's)
     const int* order = nullptr;
-    if (a.cu_q != nullptr && a.N > 1 && a.N <= kMaxOrdered && gridDim.x > a.sms) {
+    if (a.ordered) {
         make_order(a, reinterpret_cast<int*>(ring), bar.order);
         order = bar.order;
     }
@@ -430,10 +430,15 @@ int launch_latent_prompt(const fkda_latent_params& p, cudaStream_t stream, int* 
     a.H = (int)p.H;
     a.scale = p.scale;
     a.causal = p.causal;
-    a.sms = (uint32_t)device_sm_count();
     const int64_t tiles = (p.T + kRows - 1) / kRows;
     const int64_t ctas = (p.cu_seqlens != nullptr ? p.T / kRows + p.N : tiles * p.B) * p.H;   // (ragged: never fewer than there are)
     if (ctas > 0x7fffffff) return FKDA_ERR_BAD_SHAPE;
+    // The sequences with more keys first where a few rounds of SMs serve some sequences of some length: every CTA ranks all of them before
+    // its first load.  Ordered against as they come, H = 8: 8 sequences of up to 1 000 tokens 29.6 us against 31.9, of up to 4 000 131
+    // against 139, 24 of up to 1 000 62.6 against 64.0; but 12 of up to 4 000 (six rounds) 197 against 193, 24 of up to 100 16.5 against
+    // 14.4, and 512 of up to 40 took 1 180 against 250.
+    const int64_t sms = device_sm_count();
+    a.ordered = p.cu_seqlens != nullptr && p.N >= 8 && p.N <= kMaxOrdered && p.T >= 256 * p.N && ctas > sms && ctas <= 4 * sms;
     if (!allow_smem<latent_prompt_kernel>(kSmem)) return FKDA_ERR_LAUNCH;
     if (!launch_dependent(latent_prompt_kernel, ctas, kThreads, kSmem, stream, a, maps)) return FKDA_ERR_LAUNCH;
     *n_launches = 1;
