@@ -56,7 +56,8 @@ struct LinearArgs {
     int64_t q_batch, q_token, q_head, k_batch, k_token, k_head, v_batch, v_token, v_head;
     int H, group;      // value heads, value heads of a key head
     float scale;
-    bool state_fp32, skip_single;
+    bool state_fp32;
+    bool skip_single;       // the chunk kernel leaves sequences of at most one token to the step kernel (packed, no segments, not ordered)
     bool ordered;           // packed sequences: the longest first
     int seg_len, seg_rows;  // tokens of a segment, 0: every chain is walked in one piece; rows that the workspace has
     float* seg_state;       // [segment][head][128][128], and behind them
@@ -200,6 +201,12 @@ template <bool kStates, int kTerms>
 __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_constant__ LinearArgs a, const __grid_constant__ LinearMaps maps) {
     extern __shared__ __align__(1024) uint8_t smem[];
     Bars& bar = *reinterpret_cast<Bars*>(smem + kOffBars);
+    if (a.skip_single) {   // (before anything is set up: most CTAs find nothing to do)
+        grid_dep_launch();
+        grid_dep_wait();
+        int64_t first;
+        if (seq_len(a, blockIdx.x / (uint32_t)a.H, &first) <= 1) return;
+    }
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) mbar_init(&bar.full[i], 1), mbar_init(&bar.empty[i], kStates ? 1 : 2), mbar_init(&bar.dec_full[i], 1), mbar_init(&bar.dec_empty[i], kStates ? 12 : 24);
@@ -228,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     }
     const Chain ch = locate(a, row, (int)(blockIdx.x % (uint32_t)a.H));
     const bool last = ch.seg + 1 == ch.segs;
-    const bool mine = ch.len >= 0 && !(a.skip_single && ch.len <= 1) && !(kStates && last) && as_assumed(smem, bar.tmem);
+    const bool mine = ch.len >= 0 && !(kStates && last) && as_assumed(smem, bar.tmem);
     const int n = uniform(mine ? (ch.len + kC - 1) / kC : 0);
 
     if (warp == 24) {
@@ -779,10 +786,13 @@ int launch_linear(const fkda_linear_params& p, cudaStream_t stream, int* n_launc
     a.state_fp32 = p.state_dtype == FKDA_STATE_FP32;
     const int64_t chains = p.N * p.H;
     if (chains > 0x7fffffff / kStepSplit) return FKDA_ERR_BAD_SHAPE;
-    // single tokens: a fixed batch of them, or a packed batch that may hold many (the host sees only the totals): the step kernel then
-    // serves the sequences of at most one token and the chunk kernel the others
-    const bool single = p.cu_seqlens == nullptr ? p.T <= 1 : p.T < 2 * p.N;
-    const bool chunks = p.cu_seqlens == nullptr ? p.T > 1 : p.T > 1;
+    // Single tokens: a fixed batch of them, or a packed batch that must hold some (the host sees only the totals): the step kernel then
+    // serves the sequences of at most one token and the chunk kernel the others, whose CTAs find most sequences done.  Step and chunk
+    // kernel against the chunk kernel for all, 128 x 1 token, H = 32, fp32 states: 108 us against 303 (as a fixed batch 80); 64 x 1 and
+    // 64 x 2: 218 against 304; but nothing but 2 tokens: 328 against 303.  Where one round of SMs walks all chains, a single one that is
+    // longer decides: 8 x 1 and 6 tokens, H = 8, 14.1 against 10.8, nothing but single ones 6.1 against 10.5.
+    const bool single = p.cu_seqlens == nullptr ? p.T <= 1 : p.T <= p.N || (p.T < 2 * p.N && chains > device_sm_count());
+    const bool chunks = p.T > 1;
     a.skip_single = single;
     a.ordered = false;
     a.seg_len = a.seg_rows = 0;

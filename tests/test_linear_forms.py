@@ -84,3 +84,32 @@ def test_many_short_packed_sequences_cost_what_a_fixed_batch_costs(n, T, H):
         hT = torch.zeros_like(d["h0"])
         times.append(microseconds(lambda: call(d, d["h0"], hT)))
     assert times[1] < 1.5 * times[0], times
+
+
+def test_packed_single_tokens_cost_about_what_a_fixed_batch_costs():
+    """The host cannot know that no sequence is longer, so the kernel for longer ones is there too, and has to leave soon."""
+    times = []
+    for packed in (False, True):
+        d = linear_inputs([1] * 128, 32, packed=packed)
+        hT = torch.zeros_like(d["h0"])
+        times.append(microseconds(lambda: call(d, d["h0"], hT)))
+    assert times[1] < 2 * times[0], times
+
+
+@pytest.mark.parametrize("lens", [[1] * 60 + [70] + [1] * 39, [1, 0, 2] * 20 + [1] * 40, [1] * 50, [1, 0] * 40, [1, 2, 1, 1], [1, 1, 0, 1], [1] * 70 + [300, 1]],
+                         ids=lambda x: f"{len(x)} of {sum(x)}")
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16], ids=str)
+def test_single_tokens_beside_longer_sequences(lens, kind):
+    """Batches on both sides of every line between the kernels, more chains than SMs and fewer, with the state in place."""
+    H = 5
+    d = linear_inputs(lens, H, seed=22, packed=True)
+    d["h0"] = d["h0"].to(kind)
+    state = d["h0"].clone()
+    call(d, state, state)
+    at = 0
+    for n, T in enumerate(lens):
+        if T == 0:
+            assert torch.equal(state[n], d["h0"][n])
+        elif n % 3 == 0 or T > 1:
+            check_head(d, n, at, T, n % H, d["h0"], state)
+        at += T
