@@ -49,7 +49,7 @@ int check(fkda_linear_params* p) {
     if (p->state_dtype != FKDA_STATE_BF16 && p->state_dtype != FKDA_STATE_FP32) return FKDA_ERR_BAD_STATE_DTYPE;
     if (p->T > 0 && (!p->q || !p->k || !p->v || !p->g || !p->out)) return FKDA_ERR_NULL_POINTER;
     if (!aligned(p->q, 16) || !aligned(p->k, 16) || !aligned(p->v, 16) || !aligned(p->out, 16) || !aligned(p->g, 4) || !aligned(p->initial_state, 16) ||
-        !aligned(p->final_state, 16))
+        !aligned(p->final_state, 16) || !aligned(p->cu_seqlens, 8))
         return FKDA_ERR_ALIGNMENT;
     if (!tile_strides(p->q_stride, {p->B, p->T, p->Hk}) || !tile_strides(p->k_stride, {p->B, p->T, p->Hk}) || !tile_strides(p->v_stride, {p->B, p->T, p->H}) ||
         !tile_strides(p->out_stride, {p->B, p->T, p->H}))
@@ -66,7 +66,8 @@ int check(fkda_latent_params* p) {
     if (!(p->scale > 0.0f) || isinf(p->scale)) return FKDA_ERR_BAD_SCALE;
     if (p->T > 0 && (!p->q || !p->out)) return FKDA_ERR_NULL_POINTER;
     if (p->Tk > 0 && (!p->k || !p->k_rope || !p->v)) return FKDA_ERR_NULL_POINTER;
-    if (!aligned(p->q, 16) || !aligned(p->k, 16) || !aligned(p->k_rope, 16) || !aligned(p->v, 16) || !aligned(p->out, 16) || !aligned(p->lse, 4))
+    if (!aligned(p->q, 16) || !aligned(p->k, 16) || !aligned(p->k_rope, 16) || !aligned(p->v, 16) || !aligned(p->out, 16) || !aligned(p->lse, 4) ||
+        !aligned(p->cu_seqlens, 8) || !aligned(p->cu_seqlens_k, 8))
         return FKDA_ERR_ALIGNMENT;
     if (!tile_strides(p->q_stride, {p->B, p->T, p->H}) || !tile_strides(p->k_stride, {p->B, p->Tk, p->H}) || !tile_strides(p->v_stride, {p->B, p->Tk, p->H}) ||
         !tile_strides(p->k_rope_stride, {p->B, p->Tk}) || !row_strides(p->out_stride, {p->B, p->T, p->H}))

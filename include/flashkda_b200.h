@@ -205,7 +205,7 @@ int fkda_cp_fold(const float* S, const float* M, const float* N, float* out, int
 /* ---- Operators beside the KDA forward (no counterpart in the reference) ----
  *
  * Strides are in elements.  The base addresses of q, k, v, k_rope, cache and out and the strides of their dimensions longer than
- * one are positive multiples of 16 bytes; the innermost dimension is contiguous. */
+ * one are positive multiples of 16 bytes; the innermost dimension is contiguous.  Cumulative lengths are at multiples of 8 bytes. */
 
 /*
  * Linear attention with a decay for each head: S_t = exp(g_t) S_{t-1} + v_t k_t^T, o_t = scale S_t q_t.
