@@ -97,6 +97,8 @@ def lib():
             getattr(L, f"fkda_{name}_workspace_bytes").argtypes = [ctypes.POINTER(params)]
         L.fkda_operator_status.restype = ctypes.c_int
         L.fkda_operator_status.argtypes = [ctypes.c_void_p]
+        L.fkda_operator_test_starve.restype = ctypes.c_int
+        L.fkda_operator_test_starve.argtypes = [ctypes.c_int32]
         _lib = L
     return _lib
 

@@ -102,6 +102,7 @@ int launch_latent_decode(const fkda_latent_decode_params& p, cudaStream_t stream
 int linear_gave_up(cudaStream_t stream, int32_t* word);   // of the waits in each file's kernels
 int prompt_gave_up(cudaStream_t stream, int32_t* word);
 int decode_gave_up(cudaStream_t stream, int32_t* word);
+int starve_next();   // milliseconds of fkda_operator_test_starve, once
 void set_last_launch_count(int n);
 // Tensor maps over v and over the states (fkda_tc.cu).
 bool encode_v_map(CUtensorMap* m, const fkda_fwd_params& p);

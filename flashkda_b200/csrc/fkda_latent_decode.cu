@@ -54,6 +54,7 @@ struct DecodeArgs {
     int64_t out_batch, out_row, table_stride, pages;
     int B, Tq, H, R, row_tiles, groups, page, box, max_pages;
     float scale;
+    int starve_ms;       // test hook: nothing is loaded, and a wait gives up after so long
 };
 struct DecodeMaps {
     CUtensorMap q, cache;
@@ -184,6 +185,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         const int boxes = kTok / a.box;
         int g = 0, pieces = 0, asked = 0, issued[2] = {0, 0};   // (tiles of my first and second group)
         bool ok = true;
+        if (a.starve_ms > 0) starve(&bar.full[0][who], a.starve_ms, &bar.abort), ok = false;
         auto page_of = [&](int tok) {
             const int page = a.table[(int64_t)walk.b * a.table_stride + tok / a.page];
             return page < 0 || page >= a.pages ? 0 : page;
@@ -243,7 +245,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         __syncwarp();
     } else if (warp == 5) {
         // ---- products: two lines of work, each taken up as soon as what it waits for is there: the scores of tile `g`, group by group of its
-        //      dimensions, at most one tile ahead of the value product of tile `done` ----
+        //      dimensions, at most one tile ahead of the value product of tile `done`.  (It never multiplies, and so never frees, what has not
+        //      landed: the loads need no look at the abort flag.) ----
         const uint32_t q_desc = desc(smem_u32(q_smem)), k_desc = desc(smem_u32(stages)), leader = elect_one();
         const uint32_t v_desc = desc(smem_u32(stages), kChunkBytes), p_desc = desc(smem_u32(p_smem));
         // the groups that are there, from the next one on (stage and group in the code, so that the operands are constants)
@@ -606,6 +609,7 @@ int launch_latent_decode(const fkda_latent_decode_params& p, cudaStream_t stream
     a.box = p.page_size % 64 == 0 ? 64 : (p.page_size % 32 == 0 ? 32 : 16);
     a.max_pages = (int)p.max_pages;
     a.scale = p.scale;
+    a.starve_ms = starve_next();
     a.spans = reinterpret_cast<int4*>(a.parts + (int64_t)a.row_tiles * a.groups * 2 * kRows * (kValue + 1));
     DecodeMaps maps;
     const cuuint64_t qdims[3] = {(cuuint64_t)kWidth, (cuuint64_t)a.R, (cuuint64_t)p.B};

@@ -58,6 +58,7 @@ struct PromptArgs {
     bool ordered;          // packed sequences: those with more keys first
     float scale;
     int causal;
+    int starve_ms;         // test hook: nothing is loaded, and a wait gives up after so long
 };
 
 constexpr int kMaxOrdered = 32;              // packed sequences that are taken in the order of their keys
@@ -191,11 +192,13 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prompt_kernel(const __grid
     regs_dec<kRegsRest>();
     if (warp == 8) {
         // ---- loads: the queries, then for every block its keys (two tiles of the head's, one of the token's) and values ----
-        if (blocks > 0) {
+        if (a.starve_ms > 0) {
+            starve(&bar.k_full[0], a.starve_ms, &bar.abort);
+        } else if (blocks > 0) {
             const uint32_t q_addr = smem_u32(q_smem), ring_addr = smem_u32(ring), leader = elect_one();
             const int q0 = uniform((int)(p.q0 + p.row0)), row = uniform((int)p.b), k0 = uniform((int)p.k0);
             int keys = 0, values = 0;   // blocks of either that have been asked for
-            auto empty = [&](uint64_t* b, int phase) { return __all_sync(0xffffffffu, wait(b, phase & 1, &bar.abort)) != 0; };
+            auto empty = [&](uint64_t* b, int phase) { return __all_sync(0xffffffffu, wait_free(b, phase & 1, &bar.abort)) != 0; };
             auto slot = [&](int s) { return ring_addr + s * kSlotBytes; };
 #pragma unroll 1
             for (int i = 0; i < blocks; ++i) {
@@ -430,6 +433,7 @@ int launch_latent_prompt(const fkda_latent_params& p, cudaStream_t stream, int* 
     a.H = (int)p.H;
     a.scale = p.scale;
     a.causal = p.causal;
+    a.starve_ms = starve_next();
     const int64_t tiles = (p.T + kRows - 1) / kRows;
     const int64_t ctas = (p.cu_seqlens != nullptr ? p.T / kRows + p.N : tiles * p.B) * p.H;   // (ragged: never fewer than there are)
     if (ctas > 0x7fffffff) return FKDA_ERR_BAD_SHAPE;

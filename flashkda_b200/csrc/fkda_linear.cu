@@ -62,6 +62,7 @@ struct LinearArgs {
     int seg_len, seg_rows;  // tokens of a segment, 0: every chain is walked in one piece; rows that the workspace has
     float* seg_state;       // [segment][head][128][128], and behind them
     float* seg_decay;       // [segment][head]
+    int starve_ms;          // test hook: nothing is loaded, and a wait gives up after so long
 };
 struct LinearMaps {
     CUtensorMap q, k, v, out;
@@ -243,9 +244,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         const uint32_t base = smem_u32(smem), leader = elect_one();
         const int t0 = uniform((int)ch.t0), row = uniform((int)ch.b), head = uniform(ch.h), key_head = uniform(ch.h / a.group);
         int c = 0, stage = 0, phase = 1;
+        if (a.starve_ms > 0) starve(&bar.full[0], a.starve_ms, &bar.abort), c = n;
 #pragma unroll 1
         for (; c < n; ++c) {
-            if (c >= kStages && !__all_sync(0xffffffffu, wait(&bar.empty[stage], phase, &bar.abort))) break;
+            if (c >= kStages && !__all_sync(0xffffffffu, wait_free(&bar.empty[stage], phase, &bar.abort))) break;
             const uint32_t dst = base + stage * kStageBytes;
             expect(&bar.full[stage], kStates ? 2 * kOperandBytes : kStageBytes, leader);
 #pragma unroll
@@ -257,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
             if (++stage == kStages) stage = 0, phase ^= 1;
         }
 #pragma unroll 1
-        for (int k = max(0, c - kStages); k < c; ++k) drain(&bar.full[k % kStages], (k / kStages) & 1);
+        for (int k = a.starve_ms > 0 ? c : max(0, c - kStages); k < c; ++k) drain(&bar.full[k % kStages], (k / kStages) & 1);
         __syncwarp();
     } else if (warp == 25) {
         // ---- products of the state, which the next chunk waits for, and scores ----
@@ -797,6 +799,7 @@ int launch_linear(const fkda_linear_params& p, cudaStream_t stream, int* n_launc
     a.ordered = false;
     a.seg_len = a.seg_rows = 0;
     a.seg_state = a.seg_decay = nullptr;
+    a.starve_ms = starve_next();
     int launches = 0;
     if (single) {
         if (!launch_dependent(linear_step_kernel, chains * kStepSplit, 128, 0, stream, a)) return FKDA_ERR_LAUNCH;

@@ -96,7 +96,15 @@ int workspace_missing(const Params& p, size_t need) {
     return need > 0 && (p.workspace == nullptr || p.workspace_bytes < need || !aligned(p.workspace, 256)) ? FKDA_ERR_WORKSPACE : FKDA_OK;
 }
 
+thread_local int g_starve_ms = 0;
+
 }  // namespace
+
+int fkda::starve_next() {
+    const int ms = g_starve_ms;
+    g_starve_ms = 0;
+    return ms;
+}
 
 extern "C" {
 
@@ -139,6 +147,12 @@ int fkda_latent_attention_decode(const fkda_latent_decode_params* given, void* s
     rc = workspace_missing(p, fkda_latent_decode_workspace_bytes(&p));
     if (rc != FKDA_OK) return rc;
     return enqueue([&](int* n) { return fkda::launch_latent_decode(p, static_cast<cudaStream_t>(stream), n); });
+}
+
+int fkda_operator_test_starve(int32_t wait_ms) {
+    if (!in_range(wait_ms, 1, 1000)) return FKDA_ERR_BAD_SHAPE;
+    g_starve_ms = wait_ms;
+    return FKDA_OK;
 }
 
 int fkda_operator_status(void* stream_v) {

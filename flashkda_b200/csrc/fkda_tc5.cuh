@@ -12,8 +12,8 @@ namespace tc5 {
 using namespace sm100;
 
 // ------------------------------------------------------------------ waits ----
-// Every wait of these kernels is bounded.  One that gives up raises the CTA's abort flag, at which the other waits of the CTA
-// return at once: copies end, the other roles run to their ends on whatever is in shared memory (all accesses in bounds), what is
+// Every wait of these kernels is bounded.  One that gives up raises the CTA's abort flag, at which the other waits of the CTA return
+// soon: no more copies are issued, the other roles run to their ends on whatever is in shared memory (all accesses in bounds), what is
 // in flight is waited for, tensor memory is freed, and the word below tells the host (fkda_operator_status).
 static __device__ int32_t g_gave_up = 0;
 // The limit is counted in SM cycles (two seconds at 2 GHz): the global timer is far away, and reading it in the waits of a dozen
@@ -59,6 +59,19 @@ static __device__ FKDA_WAIT_INLINE bool give_up(int* abort_flag) {
 }
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* abort_flag) {
     return wait_until(bar, parity, abort_flag) || give_up(abort_flag);
+}
+// For a stage that the next copies go to.  A role that has given up runs on and frees stages whose last copies may still be on their way;
+// their barrier must not be armed a second time in one phase, so no more copies are issued then.
+__device__ __forceinline__ bool wait_free(uint64_t* bar, uint32_t parity, int* abort_flag) {
+    return wait(bar, parity, abort_flag) && *reinterpret_cast<volatile int*>(abort_flag) == 0;
+}
+// TEST ONLY: what a loading warp does in a call that is to starve: nothing is loaded, its own wait for the first tile runs out after so many
+// milliseconds (at some 2 cycles per ns), and the other roles' waits end by the flag.
+static __device__ __noinline__ void starve(uint64_t* bar, int ms, int* abort_flag) {
+    const long long start = clock64();
+    while (!mbar_try_wait(bar, 0) && clock64() - start < ms * 2000000ll) {}
+    give_up(abort_flag);
+    __syncwarp();
 }
 // The same for a whole warp, whose lanes leave it together: what follows may be an access to tensor memory or another instruction that
 // a warp executes as one.

@@ -280,6 +280,10 @@ int fkda_latent_attention_decode(const fkda_latent_decode_params* p, void* strea
  * the last call of this function (its outputs are then not to be used).  Synchronises the stream. */
 int fkda_operator_status(void* stream);
 
+/* TEST ONLY: in the next call of an operator above on this thread no kernel loads its tiles, and its waits for them give up after wait_ms
+ * (1 to 1000) milliseconds.  The call's outputs, its final state among them, are undefined. */
+int fkda_operator_test_starve(int32_t wait_ms);
+
 #ifdef __cplusplus
 }
 #endif
