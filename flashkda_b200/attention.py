@@ -99,7 +99,8 @@ def latent_decode_workspace_size(B: int, Tq: int, H: int) -> int:
 
 
 def operator_status(device=None) -> int:
-    """Synchronises the current stream of ``device`` and returns 0, or the status code of a kernel of these operators that gave up on
-    one of its bounded internal waits since the last call (see ``device_status`` for ``fwd``)."""
+    """Synchronises the current stream of ``device`` and returns 0, or the status code of a kernel of these operators, on whatever stream
+    and of whatever thread, that gave up on one of its bounded internal waits there since this thread last asked (the first time: since the
+    library was loaded; see ``device_status`` for ``fwd``)."""
     with torch.cuda.device(device):
         return int(_lib.lib().fkda_operator_status(torch.cuda.current_stream().cuda_stream))

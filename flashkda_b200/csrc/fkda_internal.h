@@ -99,9 +99,9 @@ int launch_linear(const fkda_linear_params& p, cudaStream_t stream, int* n_launc
 int launch_latent_prompt(const fkda_latent_params& p, cudaStream_t stream, int* n_launches);
 size_t latent_decode_workspace(const fkda_latent_decode_params& p);
 int launch_latent_decode(const fkda_latent_decode_params& p, cudaStream_t stream, int* n_launches);
-int linear_gave_up(cudaStream_t stream, int32_t* word);   // of the waits in each file's kernels
-int prompt_gave_up(cudaStream_t stream, int32_t* word);
-int decode_gave_up(cudaStream_t stream, int32_t* word);
+int linear_gave_up(cudaStream_t stream, uint32_t* times);   // waits in each file's kernels, on the current device
+int prompt_gave_up(cudaStream_t stream, uint32_t* times);
+int decode_gave_up(cudaStream_t stream, uint32_t* times);
 int starve_next();   // milliseconds of fkda_operator_test_starve, once
 void set_last_launch_count(int n);
 // Tensor maps over v and over the states (fkda_tc.cu).

@@ -634,6 +634,6 @@ int launch_latent_decode(const fkda_latent_decode_params& p, cudaStream_t stream
     return FKDA_OK;
 }
 
-int decode_gave_up(cudaStream_t stream, int32_t* word) { return read_gave_up(stream, word); }
+int decode_gave_up(cudaStream_t stream, uint32_t* times) { return read_gave_up(stream, times); }
 
 }  // namespace fkda

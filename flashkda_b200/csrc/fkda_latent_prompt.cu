@@ -449,6 +449,6 @@ int launch_latent_prompt(const fkda_latent_params& p, cudaStream_t stream, int* 
     return FKDA_OK;
 }
 
-int prompt_gave_up(cudaStream_t stream, int32_t* word) { return read_gave_up(stream, word); }
+int prompt_gave_up(cudaStream_t stream, uint32_t* times) { return read_gave_up(stream, times); }
 
 }  // namespace fkda

@@ -845,6 +845,6 @@ int launch_linear(const fkda_linear_params& p, cudaStream_t stream, int* n_launc
     return FKDA_OK;
 }
 
-int linear_gave_up(cudaStream_t stream, int32_t* word) { return read_gave_up(stream, word); }
+int linear_gave_up(cudaStream_t stream, uint32_t* times) { return read_gave_up(stream, times); }
 
 }  // namespace fkda

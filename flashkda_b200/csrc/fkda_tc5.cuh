@@ -14,8 +14,8 @@ using namespace sm100;
 // ------------------------------------------------------------------ waits ----
 // Every wait of these kernels is bounded.  One that gives up raises the CTA's abort flag, at which the other waits of the CTA return
 // soon: no more copies are issued, the other roles run to their ends on whatever is in shared memory (all accesses in bounds), what is
-// in flight is waited for, tensor memory is freed, and the word below tells the host (fkda_operator_status).
-static __device__ int32_t g_gave_up = 0;
+// in flight is waited for, tensor memory is freed, and the count below tells the host (fkda_operator_status).
+static __device__ uint32_t g_gave_up = 0;
 // The limit is counted in SM cycles (two seconds at 2 GHz): the global timer is far away, and reading it in the waits of a dozen
 // warps made all of them slower.
 constexpr long long kWaitCycles = 4000000000ll;
@@ -42,19 +42,16 @@ __device__ __forceinline__ bool wait_until(uint64_t* bar, uint32_t parity, volat
     return mbar_try_wait(bar, parity) || wait_on(bar, parity, abort_flag);
 }
 
-// The word of this translation unit's kernels, once the stream has come this far; cleared for the next reader.
-static int read_gave_up(cudaStream_t stream, int32_t* word) {
-    const int32_t zero = 0;
-    if (cudaMemcpyFromSymbolAsync(word, g_gave_up, sizeof(*word), 0, cudaMemcpyDeviceToHost, stream) != cudaSuccess ||
-        cudaStreamSynchronize(stream) != cudaSuccess)
-        return FKDA_ERR_LAUNCH;
-    if (*word != 0 && cudaMemcpyToSymbolAsync(g_gave_up, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, stream) != cudaSuccess) return FKDA_ERR_LAUNCH;
-    return FKDA_OK;
+// How often this translation unit's kernels have given up on the current device, once the stream has come this far.  Only ever counted
+// up: several threads may ask, and kernels on other streams may give up meanwhile.
+static int read_gave_up(cudaStream_t stream, uint32_t* times) {
+    const bool read = cudaMemcpyFromSymbolAsync(times, g_gave_up, sizeof(*times), 0, cudaMemcpyDeviceToHost, stream) == cudaSuccess;
+    return read && cudaStreamSynchronize(stream) == cudaSuccess ? FKDA_OK : FKDA_ERR_LAUNCH;
 }
 
 static __device__ FKDA_WAIT_INLINE bool give_up(int* abort_flag) {
     *reinterpret_cast<volatile int*>(abort_flag) = 1;
-    g_gave_up = 1;
+    atomicAdd(&g_gave_up, 1u);
     return false;
 }
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* abort_flag) {
@@ -215,7 +212,7 @@ __device__ __forceinline__ void st_frag8(uint32_t taddr, uint32_t r0, uint32_t r
 // at 0 where a CTA has all of it: then addresses and descriptors are constants.  (Never seen otherwise; checked all the same.)
 __device__ __forceinline__ bool as_assumed(const void* smem, uint32_t tmem) {
     if ((smem_u32(smem) & 1023u) == 0 && tmem == 0) return true;
-    g_gave_up = 1;
+    atomicAdd(&g_gave_up, 1u);
     return false;
 }
 

@@ -276,8 +276,9 @@ typedef struct fkda_latent_decode_params {
 size_t fkda_latent_decode_workspace_bytes(const fkda_latent_decode_params* p);
 int fkda_latent_attention_decode(const fkda_latent_decode_params* p, void* stream);
 
-/* FKDA_OK, or FKDA_ERR_DEVICE_STATUS if a kernel of the operators above gave up on a bounded wait on the current device since
- * the last call of this function (its outputs are then not to be used).  Synchronises the stream. */
+/* FKDA_OK, or FKDA_ERR_DEVICE_STATUS if a kernel of the operators above gave up on a bounded wait on the current device, whatever its stream
+ * and thread, since this thread last asked there (or, the first time, since the library was loaded): outputs of that time are then not
+ * to be used.  Synchronises the stream. */
 int fkda_operator_status(void* stream);
 
 /* TEST ONLY: in the next call of an operator above on this thread no kernel loads its tiles, and its waits for them give up after wait_ms

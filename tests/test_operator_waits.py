@@ -4,6 +4,7 @@ Every wait has a limit.  When it runs out the kernel stops loading, lets its rol
 what is in flight and returns; ``operator_status`` then reports it.  A test-only hook makes that happen without any fault: one call
 loads nothing, and the first wait for its tiles has a limit of a few milliseconds.
 """
+import threading
 import time
 
 import pytest
@@ -11,7 +12,7 @@ import torch
 
 import flashkda_b200 as lib
 from flashkda_b200 import _lib
-from test_attention_calls import CALLS, chunk_call, decode_call, prompt_call, results
+from test_attention_calls import CALLS, chunk_call, decode_call, results
 
 gpu = pytest.mark.gpu
 WAITING = sorted(set(CALLS) - {"step"})
@@ -52,3 +53,32 @@ def test_the_hook_is_for_one_call_on_its_thread():
     torch.cuda.synchronize()
     assert all(torch.equal(o, w) for o, w in zip(outs, want))
     assert lib.operator_status() == 9 and lib.operator_status() == 0
+
+
+@gpu
+def test_every_thread_is_told():
+    """A thread that asks first does not take the report away from another, nor does one that asks again get it twice."""
+    call, outs = decode_call()
+    want = results(call, outs)
+    ask, answers = [threading.Event() for _ in range(2)], []
+
+    def other():
+        answers.append(lib.operator_status())      # (whatever there was before)
+        answers.append(lib.operator_status())
+        ask[0].set()
+        ask[1].wait(30)
+        answers.append(lib.operator_status())
+        answers.append(lib.operator_status())
+
+    t = threading.Thread(target=other)
+    t.start()
+    ask[0].wait(30)
+    lib.operator_status()
+    assert _lib.lib().fkda_operator_test_starve(3) == 0
+    call()
+    assert lib.operator_status() == 9 and lib.operator_status() == 0
+    ask[1].set()
+    t.join()
+    assert answers[1:] == [0, 9, 0]
+    assert all(torch.equal(a, b) for a, b in zip(results(call, outs), want))
+    assert lib.operator_status() == 0
