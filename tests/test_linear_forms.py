@@ -113,3 +113,28 @@ def test_single_tokens_beside_longer_sequences(lens, kind):
         elif n % 3 == 0 or T > 1:
             check_head(d, n, at, T, n % H, d["h0"], state)
         at += T
+
+
+# one chain per CTA in one piece; in segments of several chunks, fixed and packed; more chains than SMs, in the order of their lengths and,
+# with one sequence more than are put in order, as they come
+LONG = [([900], 80, 80, 1), ([1500, 1500], 80, 20, 1), ([8192], 32, 32, 2), ([3000, 1, 5000], 16, 4, 2), ([2000, 900, 1, 63, 1500, 700], 48, 12, 3),
+        ([340 + 7 * (i % 9) for i in range(64)], 4, 4, 5), ([350 + 7 * (i % 9) for i in range(65)], 4, 2, 5)]
+
+
+@pytest.mark.parametrize("lens,H,Hk,every", LONG, ids=[f"{len(x[0])} of {sum(x[0])} x {x[1]}" for x in LONG])
+@pytest.mark.parametrize("kind", [None, torch.float32, torch.bfloat16], ids=str)
+def test_values_over_many_chunks(lens, H, Hk, every, kind):
+    """All buffers of the walk used many times over, and states that are handed from segment to segment, against 64 bits."""
+    packed = len(set(lens)) > 1
+    d = linear_inputs(lens, H, Hk, seed=23, packed=packed, strong=0.05)
+    d["h0"] = d["h0"].to(kind or torch.float32)
+    hT = torch.full_like(d["h0"], 9.0)
+    h0 = d["h0"] if kind else None
+    call(d, h0, hT)
+    at = 0
+    for n, T in enumerate(lens):
+        if n % every == 0 or n >= len(lens) - 2:
+            for h in sorted({0, H // 2 - 1, H - 1}):
+                check_head(d, n, at, T, h, h0, hT, packed)
+        at += T
+    assert flashkda_b200.operator_status() == 0
