@@ -58,3 +58,27 @@ def test_many_short_packed_prompts_cost_about_what_a_fixed_batch_costs(n, T, H):
         d = prompts([T] * n, [0] * n, H, 1, packed)
         times.append(microseconds(lambda: call(d)))
     assert times[1] < 2.5 * times[0], times
+
+
+def uneven(n, mean, seed):
+    gen = torch.Generator().manual_seed(seed)
+    lens = torch.randint(1, 2 * mean, (n,), generator=gen).tolist()
+    return [x + max(0, mean - sum(lens) // n + 1) for x in lens], torch.randint(0, 900, (n,), generator=gen).tolist()
+
+
+# batches that are taken in the order of their keys (which is not that of their queries, has ties, and sequences without queries or
+# without a prefix), and those just outside: one sequence more or fewer, more rounds of SMs, shorter sequences
+ORDERS = {
+    "ties and empty ones": ([300, 0, 513, 300, 1, 700, 256, 130], [700, 50, 0, 700, 2000, 0, 1000, 870], 16),
+    "7": (*uneven(7, 400, 1), 16), "8": (*uneven(8, 400, 2), 16), "32": (*uneven(32, 260, 3), 8), "33": (*uneven(33, 260, 4), 8),
+    "many rounds": (*uneven(20, 300, 5), 32), "short": (*uneven(30, 40, 6), 8)}
+
+
+@pytest.mark.parametrize("name", ORDERS)
+def test_packed_prompts_in_and_out_of_order(name):
+    lens, prefix, H = ORDERS[name]
+    d = prompts(lens, prefix, H, 7)
+    call(d)
+    check_heads(d, lens, prefix, slice(0, 2))
+    check_heads(d, lens, prefix, slice(H - 1, H))
+    assert flashkda_b200.operator_status() == 0
