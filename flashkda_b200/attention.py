@@ -47,7 +47,8 @@ def linear_attention_fwd(q, k, v, g, scale, out, initial_state=None, final_state
     Sequences of more than one token go through 64-token chunks on the tensor cores; single tokens (``T == 1``, or the sequences of one
     token in a packed batch of mostly such) through one read-modify-write of the states.  In between the state is fp32, whatever its type
     in memory; what a chunk adds to it holds 24 bits, or 16 behind a bf16 ``initial_state``.  Outputs do not depend on whether a
-    ``final_state`` is asked for, nor on its type.  ``workspace``: optional caller-owned uint8 scratch for calls that need some
+    ``final_state`` is asked for, nor on its type.  An element of v that is not finite makes its dimension of out NaN from the start of its
+    chunk on, so in up to 63 tokens in front of it; of q, k and g nothing reaches an earlier token.  ``workspace``: optional caller-owned uint8 scratch for calls that need some
     (``linear_attention_workspace_size``).
     """
     _linear_attention_fwd(q, k, v, g, scale, out, initial_state, final_state, cu_seqlens, workspace)
@@ -63,8 +64,9 @@ def latent_attention_fwd(q, k, k_rope, v, scale, out, lse=None, cu_seqlens=None,
     logarithm of the softmax's sum, with which results over parts of the keys can be joined.  ``causal``: query ``i`` of ``T`` sees
     the keys ``j <= i + Tk - T`` (the last query sees all: keys in front of the queries are a cached prefix); a row that sees nothing
     gets 0 and ``lse`` minus infinity.  cu_seqlens, cu_seqlens_k: int64 ``[N + 1]`` of packed queries and keys (then ``B`` must
-    be 1); ``cu_seqlens`` serves both if it is given alone.  Rows that no sequence has are left as they were.  ``scale`` must be
-    positive.
+    be 1); ``cu_seqlens`` serves both if it is given alone.  Rows that no sequence has are left as they were.  An element of v that is
+    not finite makes its dimension of out NaN also in rows that do not see it, up to 255 in front of those that do; of k and k_rope nothing
+    reaches such rows.  ``scale`` must be positive.
     """
     _latent_attention_fwd(q, k, k_rope, v, scale, out, lse, cu_seqlens, cu_seqlens_k, causal)
 
@@ -81,7 +83,8 @@ def latent_attention_decode(q, cache, block_table, cache_lens, scale, out, lse=N
     tokens in the cache, the new ones among them; out: bf16 ``[B, Tq, H, 512]``; lse: fp32 ``[B, Tq, H]``.  New token ``i`` sees the
     first ``len - Tq + 1 + i`` tokens; one that sees none gets 0 and ``lse`` minus infinity.  In q and out the new tokens lie ``H``
     heads apart.  What a page holds behind a sequence's last token is not used; entries of ``block_table`` that are no page number
-    read page 0.  At most 36 864 sequences; ``scale`` must be positive.  ``workspace``: optional caller-owned uint8 scratch
+    read page 0.  A cached number among a token's first 512 that is not finite makes its dimension of out NaN for all ``Tq`` tokens of its
+    sequence, those that do not see it as well.  At most 36 864 sequences; ``scale`` must be positive.  ``workspace``: optional caller-owned uint8 scratch
     (``latent_decode_workspace_size``).
     """
     _latent_attention_decode(q, cache, block_table, cache_lens, scale, out, lse, workspace)
