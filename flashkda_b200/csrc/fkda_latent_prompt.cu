@@ -53,7 +53,7 @@ struct PromptArgs {
     __nv_bfloat16* out;
     float* lse;
     const int64_t *cu_q, *cu_k;
-    int64_t B, T, Tk, N, out_batch, out_token, out_head;
+    int64_t T, Tk, N, out_batch, out_token, out_head;
     int H;
     bool ordered;          // packed sequences: those with more keys first
     float scale;
@@ -428,7 +428,7 @@ int launch_latent_prompt(const fkda_latent_params& p, cudaStream_t stream, int* 
     a.lse = p.lse;
     a.cu_q = p.cu_seqlens;
     a.cu_k = p.cu_seqlens_k;
-    a.B = p.B; a.T = p.T; a.Tk = p.Tk; a.N = p.N;
+    a.T = p.T; a.Tk = p.Tk; a.N = p.N;
     a.out_batch = p.out_stride[0]; a.out_token = p.out_stride[1]; a.out_head = p.out_stride[2];
     a.H = (int)p.H;
     a.scale = p.scale;

@@ -115,12 +115,6 @@ __device__ __forceinline__ void load_3d(uint32_t dst, const void* tmap, int c0, 
         "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar)), "r"(leader)
         : "memory");
 }
-// The same tile into L2 only, ahead of its load.
-__device__ __forceinline__ void prefetch_3d(const void* tmap, int c0, int c1, int c2, uint32_t leader) {
-    asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %4, 0;\n@q cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];\n}\n" ::"l"(tmap), "r"(c0), "r"(c1), "r"(c2),
-                 "r"(leader)
-                 : "memory");
-}
 __device__ __forceinline__ void tma_store_4d(const void* tmap, int c0, int c1, int c2, int c3, const void* smem_src) {
     asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(tmap), "r"(c0), "r"(c1), "r"(c2),
                  "r"(c3), "r"(smem_u32(smem_src))
