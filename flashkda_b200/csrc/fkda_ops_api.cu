@@ -1,5 +1,5 @@
 // C ABI of the operators beside the KDA forward: argument validation in front of the launches.
-#include <math.h>
+#include <float.h>
 
 #include <array>
 #include <initializer_list>
@@ -30,6 +30,9 @@ bool row_strides(const int64_t* stride, std::initializer_list<int64_t> sizes) {
     }
     return true;
 }
+// Kernels multiply scores, masked ones of minus infinity among them, by scale times log2(e), which therefore is neither 0 (where a smaller
+// number would be flushed to) nor infinite.
+bool softmax_scale(float x) { return x >= FLT_MIN && x <= FLT_MAX / 2; }
 bool in_range(int64_t x, int64_t lo, int64_t hi) { return lo <= x && x <= hi; }
 constexpr int64_t kMost = 0x7fffffff;
 
@@ -64,7 +67,7 @@ int check(fkda_latent_params* p) {
     if ((p->cu_seqlens != nullptr) != (p->cu_seqlens_k != nullptr)) return FKDA_ERR_NULL_POINTER;
     if (p->cu_seqlens != nullptr && p->B != 1) return FKDA_ERR_VARLEN_BATCH;
     if (p->cu_seqlens == nullptr && p->N != p->B) return FKDA_ERR_BAD_SHAPE;
-    if (!(p->scale > 0.0f) || isinf(p->scale)) return FKDA_ERR_BAD_SCALE;
+    if (!softmax_scale(p->scale)) return FKDA_ERR_BAD_SCALE;
     if (p->T > 0 && (!p->q || !p->out)) return FKDA_ERR_NULL_POINTER;
     if (p->Tk > 0 && (!p->k || !p->k_rope || !p->v)) return FKDA_ERR_NULL_POINTER;
     if (!aligned(p->q, 16) || !aligned(p->k, 16) || !aligned(p->k_rope, 16) || !aligned(p->v, 16) || !aligned(p->out, 16) || !aligned(p->lse, 4) ||
@@ -81,7 +84,7 @@ int check(fkda_latent_decode_params* p) {
         !in_range(p->pages, 0, kMost) || !in_range(p->page_size, 16, 1 << 20) || p->page_size % 16 != 0 || !in_range(p->max_pages, 0, kMost) ||
         p->max_pages * p->page_size > kMost - 64)
         return FKDA_ERR_BAD_SHAPE;
-    if (!(p->scale > 0.0f) || isinf(p->scale)) return FKDA_ERR_BAD_SCALE;
+    if (!softmax_scale(p->scale)) return FKDA_ERR_BAD_SCALE;
     if (p->B * p->Tq == 0) return FKDA_OK;
     if (!p->q || !p->cache_lens || !p->out || (p->max_pages > 0 && (!p->block_table || !p->cache)) || (p->max_pages > 0 && p->pages < 1)) return FKDA_ERR_NULL_POINTER;
     if (!aligned(p->q, 16) || !aligned(p->cache, 16) || !aligned(p->out, 16) || !aligned(p->lse, 4) || !aligned(p->block_table, 4) || !aligned(p->cache_lens, 4))
