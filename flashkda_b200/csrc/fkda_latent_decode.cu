@@ -14,9 +14,10 @@
 // value product as it lies (dimension-major), and 256 of the 512 tensor-memory columns are enough.
 //
 // Measured: a tile of 64 tokens takes a CTA some 2 300 cycles of products (36 of 64 x 64 at 42, 16 of 128 x 64 at 49) and 1 100 of weights,
-// which run beside the next tile's scores, against 3 100 for its bytes: 64 sequences of 4 000 tokens of 64 heads walk at the copy
-// bandwidth; the listed batch of 128 uneven ones takes 153 to 172 us with its start, its outputs and the joining (0.64 to 0.57 of the copy
-// bandwidth).  384 rows per token: 321 to 340 us, 0.42 of cuBLAS.  One sequence of 2 989 tokens: 14 us, of which 6.5 are the walk.
+// which run beside the next tile's scores, against 3 100 for its bytes, and yet some 4 500 in all: neither HBM (59 % of its peak) nor the tensor
+// cores (46 %) bound the walk.  148 sequences of 4 096 tokens of 64 heads 148 us, 0.72 of the copy bandwidth; 64 of 4 000, most of them cut,
+// 89 to 98 (0.51 to 0.46); 128 uneven ones up to 8 192 165 to 174 in passes back to back, 153 in short runs (0.59 to 0.56, 0.64).  384 rows
+// per token: 335 to 342 us, 321 in short runs, 0.40 of cuBLAS.  One sequence of 2 989 tokens: 14 us, of which 6.5 are the walk.
 //
 // Numerics: as in the expanded form (fp32 scores, sums and outputs; weights against a reference within 2^8 of the running maximum,
 // rounded to bf16 for the value product only); parts are joined in fp32 in the order of the tokens.
@@ -81,8 +82,7 @@ __device__ __forceinline__ int length(const DecodeArgs& a, int b) {
 struct Walk {
     int b, t, left;
     int len, tiles, until;   // of the current stretch: [t, until)
-    // (Not inlined: with its loop in sight the compiler no longer sees the warps as converged, and the descriptors of the products leave
-    // the uniform registers.)
+    // (Not inlined: inlined, such a loop made the products slower, as it did in the prompts' kernel.)
     __device__ __noinline__ bool next(const DecodeArgs& a) {
         if (left <= 0) return false;
         len = length(a, b);

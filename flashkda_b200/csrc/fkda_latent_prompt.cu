@@ -9,8 +9,9 @@
 // (128 tokens x 64 dimensions); the rotated part needs no copy beside the others: it is the third tile of a key block, read
 // through a map of its own.  Packed sequences with more keys are taken first.
 //
-// Measured: 8 192 tokens of 32 heads 516 us, 1.33 PFLOP/s (0.79 of cuBLAS in a burst); 595, 0.84 of what cuBLAS sustains, where the power
-// cap holds the clock.
+// Measured: 8 192 tokens of 32 heads 595 to 615 us, 0.84 to 0.81 of what cuBLAS sustains, where the power cap holds the clock (passes back
+// to back for some tenths of a second); 516 us, 1.33 PFLOP/s, 0.79 of cuBLAS in a burst, in short runs at 1.9 GHz, in which the other
+// times below were taken.
 // A pair of tiles takes 3 160 cycles per block of keys, for 2 560 of tensor-core work and 2 048 of exponentials; a tile's own
 // chain, scores to weights (1 680) to product and the next scores (1 020), with 390 between them, is as long.  One thread's instruction
 // stream feeds the tensor cores, so what it has to do beside products counts: barriers per block instead of per 16 KB tile made
@@ -130,8 +131,8 @@ __device__ __forceinline__ Place locate(const PromptArgs& a, const int* order, i
     return p;
 }
 
-// (Not inlined: with its loops in sight the compiler no longer sees the warps as converged, and the descriptors of the products leave the
-// uniform registers: 546 -> 960 us for 8 192 tokens of 32 heads.)
+// (Not inlined: inlined it made 960 us of 546 for 8 192 tokens of 32 heads; probably the compiler no longer knows then that the warps
+// are converged.)
 __device__ __noinline__ void make_order(const PromptArgs& a, int* lens, int* order) {
     for (int i = threadIdx.x; i < a.N; i += kThreads) lens[i] = (int)(a.cu_k[i + 1] - a.cu_k[i]);
     fence_proxy_async_smem();

@@ -18,12 +18,16 @@
 // piece 205.
 //
 // Numerics: decays are sums of g in fp32 over at most 64 tokens, w as sums over the tokens behind j (no differences of large sums).
-// P and the copy of S that Q multiplies are rounded to bf16, which the bf16 outputs do not show.  The state is not rounded: it
-// is fp32 throughout, and w V enters the product as three bf16 terms, which hold all 24 bits; as two, which hold 16, where the
-// initial state is bf16 (half a step of its own is 2^-8, of the terms 2^-16; 6 % less time where the power cap rules).
+// P and the copy of S that Q multiplies are operands of products and rounded to bf16 for them: bf16 outputs are 2.35e-3 from 64 bits
+// (2-norm), where their own rounding alone is 1.66e-3.  The state is not rounded: it is fp32 throughout, and w V enters the product as three bf16 terms, which hold all 24 bits; as two, which hold 16, where the
+// initial state is bf16 (half a step of its own is 2^-8, of the terms 2^-16; 6 % less time where the power cap rules).  The tensor cores
+// cut fp32 sums off where an addition elsewhere would round, twelve times a chunk, so an fp32 state comes out low by what its memory
+// gathers: 1.3e-7 of it for decays of exp(-1), 4e-7 for exp(-1/64), 1.3e-6 for exp(-1/256), 4.5e-6 for exp(-1/1024), 2.7e-5 for
+// exp(-1/8192) over 16 384 tokens.
 //
 // Single tokens: a read-modify-write of the state by a kernel of its own, as bound by HBM as that is (256 x 64 states in bf16: 172 to
-// 190 us, 0.97 to 0.87 of the copy bandwidth; one sequence: the launch, 2.6 to 3.2 us).
+// 190 us, 0.97 to 0.87 of the copy bandwidth; one sequence: the launch, 2.6 to 3.2 us).  Of a packed batch the host does not know that all
+// sequences are such, and the chunk kernel's CTAs, one to an SM, have to come and see: 294 us for the same 256 x 64 states.
 #include "fkda_tc5.cuh"
 
 namespace fkda {
@@ -99,8 +103,8 @@ __device__ __forceinline__ int seq_len(const LinearArgs& a, int64_t n, int64_t* 
     return hi > lo ? (int)(hi - lo) : 0;
 }
 __device__ __forceinline__ int segments(const LinearArgs& a, int len) { return a.seg_len == 0 || len == 0 ? 1 : (len + a.seg_len - 1) / a.seg_len; }
-// (Not inlined, nor is the next one: with their loops in sight the compiler no longer sees the warps as converged, and the descriptors
-// of the products leave the uniform registers.)
+// (Not inlined, nor is the next one: inlined, such searches made the products slower, as they did in the prompts' kernel; probably the
+// compiler no longer knows then that the warps are converged.)
 // `row`: of (sequence, segment) pairs in order; len < 0: there are fewer.
 __device__ __noinline__ Chain locate(const LinearArgs& a, int64_t row, int h) {
     Chain c;

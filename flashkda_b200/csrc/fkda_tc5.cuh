@@ -252,9 +252,9 @@ __host__ __device__ constexpr uint32_t idesc(int M, int N, bool a_mn, bool b_mn)
     return (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
            ((uint32_t)(M >> 4) << 24);
 }
-// Products are issued by ONE thread, but a whole warp runs the code around them, with the same values in all lanes: then descriptors are
-// uniform registers, and an instruction goes out every 32 to 64 cycles (what its operands take) instead of every 75 (A in tensor memory)
-// or 116.  `leader` is 1 in the lane that issues.
+// Products are issued by ONE thread, but a whole warp runs the code around them, with the same values in all lanes: measured so, an
+// instruction goes out every 32 to 64 cycles (what its operands take) instead of every 75 (A in tensor memory) or 116, probably because
+// descriptors then need not be moved for each.  `leader` is 1 in the lane that issues.
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
 // D[tmem] (+)= A[smem] B[smem], K = 16; accumulate = 0 overwrites D.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t accumulate, uint32_t leader) {
