@@ -828,9 +828,10 @@ int launch_linear(const fkda_linear_params& p, cudaStream_t stream, int* n_launc
         // The longest first where not all run at once and the last ones are worth what it costs: every CTA ranks all sequences before its
         // first load, 1 us and 0.03 us per sequence.  Ordered against as they come, H = 16: 16 sequences of up to 4 000 tokens 123 us
         // against 156, of up to 1 000 tokens 59 against 67, 32 of these 118 against 117, 64 of these 205 against 195; of up to 60 tokens 16
-        // take 27 against 24, 96 168 against 128, and 896 of up to 400 took 5.9 ms against 1.45.
+        // take 27 against 24, 96 168 against 128, and 896 of up to 400 took 5.9 ms against 1.45.  4 to 48 sequences, 1.1 to 4.5 rounds
+        // of SMs: 0.74 to 0.97 of the time from 240 tokens per sequence and round on, 0.93 to 1.03 from 160 on, 1.05 to 1.2 below 60.
         const int64_t sms = device_sm_count();
-        a.ordered = p.cu_seqlens != nullptr && seg.len == 0 && p.N > 1 && p.N <= kMaxOrdered && chains > sms && p.T >= 192 * p.N * chains / sms;
+        a.ordered = p.cu_seqlens != nullptr && seg.len == 0 && p.N > 1 && p.N <= kMaxOrdered && chains > sms && p.T >= 160 * p.N * chains / sms;
         // (by the initial state alone: outputs do not depend on whether, and in which type, a final state is asked for)
         const bool exact = a.state_fp32 || p.initial_state == nullptr;
         auto walk = [&](bool states) {
