@@ -622,6 +622,9 @@ int launch_latent_decode(const fkda_latent_decode_params& p, cudaStream_t stream
     maps.cache = maps.q;   // (where there is no page, nothing is read)
     if (p.pages > 0 && p.max_pages > 0 && !encode_bf16_map(&maps.cache, 3, p.cache, cdims, cstrides, cbox)) return FKDA_ERR_LAUNCH;
     const int ctas = a.row_tiles * a.groups;
+    // Both shapes, one row a CTA against four: 16 sequences of 32 heads (512 rows) up to 3 000 tokens 26.2 us against 35.1, one of 64
+    // heads up to 20 000 19.8 against 71.5; 64 of 16 heads (1 024 rows) 58.8 against 53.4, 16 of 64 heads (1 024) 34.9 against 37.9; 32 of
+    // 64 heads (2 048) 58.4 against 47.6, 64 of 128 heads (8 192) 169 against 90.
     const int rows_each = p.B * a.R > 4 * device_sm_count() ? 4 : 1, per = (a.R + rows_each - 1) / rows_each;
     const int64_t joins = p.B * per;
     if (joins > 0x7fffffff) return FKDA_ERR_BAD_SHAPE;
